@@ -301,6 +301,73 @@ void kmi_gemm_force_tile(int tile);
 void kmi_gemm_force_splits(int splits);
 void kmi_gemm_force_group_m(int group_m);
 
+/* ---- rotary positions, paged key-value cache, decode attention ---------------------------------------- */
+
+/* The operators between a decoder layer's qkv linear and its output linear.  The reference leaves them to the host
+ * framework's modules (kairos/main.py:141 runs stock decoder layers); nothing here replaces one of its functions.
+ *
+ * A cache is [num_pages][KV][page_tiles][tile bytes], zeroed or not; a page holds 32 * page_tiles tokens.  A tile is 32
+ * consecutive tokens of one key head: keys, values, fp16 factors, in the lane order of the MFMA that reads them
+ * (kairos_amd/csrc/kv_parts.h).  kind: KMI_KV_F16 stores elements; KMI_KV_INT8 codes u and one scale s a row,
+ * s * (u - 128); KMI_KV_INT4 codes and a scale and an offset a row, s * u + z.  page_table is int32 [B][max_pages]: position
+ * t of sequence b lies in page page_table[b][t / (32 * page_tiles)].  Entries outside [0, num_pages) are never followed:
+ * what would be written there is dropped, what would be read from there comes back as NaN.
+ * The structs are plain in-parameters: they are read during the call and not kept. */
+#define KMI_KV_F16 0
+#define KMI_KV_INT8 1
+#define KMI_KV_INT4 2
+int kmi_kv_tile_bytes(int D, int kind);     /* bytes of a tile, or KMI_E_SHAPE; D = 64, 128 or 256 */
+
+/* Token s of sequence b stands at position start[b] + s.  Rotates the first rotary_dim elements of every query and key head
+ * by table [table_rows][rotary_dim / 2][2] (fp32 cosine, sine; a position outside it gives NaN), pairs (i, i + rotary_dim/2),
+ * or (2i, 2i+1) with `interleaved`; rotary_dim 0 = no rotation.  Writes q_out (with q), k_out (if not NULL) and, with a
+ * cache, the rotated keys and the values of the tokens' positions.  Tokens s >= count[b] (count may be NULL: none) are
+ * padding: zeros in q_out / k_out, nothing in the cache.  q, k, v: fp16 [B][S][heads][D] with element strides for B and S
+ * (multiples of 8), heads contiguous; outputs contiguous.  No two tokens of a call may share a place in the cache. */
+typedef struct {
+    void* q_out;
+    void* k_out;
+    void* cache;
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* table;
+    const int32_t* start;
+    const int32_t* count;
+    const int32_t* page_table;
+    int64_t q_batch, q_token, k_batch, k_token, v_batch, v_token;
+    int32_t B, S, H, KV, D, rotary_dim, table_rows, interleaved, kind, num_pages, page_tiles, max_pages;
+} kmi_rope_kv_args;
+int kmi_rope_kv(const kmi_rope_kv_args* args, void* stream);
+
+/* k_out, v_out fp16 [B][S][KV][D] <- what the cache holds for positions start[b] .. start[b] + S - 1, each value rounded to
+ * fp16 once (and kept finite); zeros for s >= count[b]. */
+typedef struct {
+    void* k_out;
+    void* v_out;
+    const void* cache;
+    const int32_t* start;
+    const int32_t* count;
+    const int32_t* page_table;
+    int32_t B, S, KV, D, kind, num_pages, page_tiles, max_pages;
+} kmi_kv_read_args;
+int kmi_kv_read(const kmi_kv_read_args* args, void* stream);
+
+/* out fp16 [B][H][D] <- softmax(scale q . K) V over positions max(0, lens[b] - window) .. lens[b] - 1 (window 0: from 0) of the
+ * cache, H a multiple of KV, query head h on key head h / (H / KV); q fp16 [B][H][D] with an element stride for B.  A sequence
+ * of no tokens gives zeros; one longer than its row of the page table gives NaN. */
+typedef struct {
+    void* out;
+    const void* q;
+    const void* cache;
+    const int32_t* page_table;
+    const int32_t* lens;
+    int64_t q_batch;
+    float scale;
+    int32_t B, H, KV, D, kind, num_pages, page_tiles, max_pages, window;
+} kmi_paged_attn_args;
+int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream);
+
 /* ---- interval lookup table (host only) --------------------------------------------------------- */
 
 /* Replaces LUT_module.LUT (kernels/csrc/kairos_kernel/lut/lut.h:8-45, lut_bindings.cpp:5-13).

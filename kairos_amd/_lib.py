@@ -55,6 +55,11 @@ SIGNATURES = {
     "kmi_gemm_splits_for": [_I, _I, _I, _I, _Z],
     "kmi_gemm_force_splits": [_I],
     "kmi_gemm_force_group_m": [_I],
+    # (pointer to a struct of arguments, stream); kmi_kv_tile_bytes is host arithmetic
+    "kmi_kv_tile_bytes": [_I, _I],
+    "kmi_rope_kv": [ctypes.c_char_p, _P],
+    "kmi_kv_read": [ctypes.c_char_p, _P],
+    "kmi_paged_attn": [ctypes.c_char_p, _P],
     "kmi_lut_new": [],
     "kmi_lut_free": [_P],
     "kmi_lut_record": [_P, _I, _I],

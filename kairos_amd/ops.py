@@ -4,6 +4,7 @@ replace (kernels/csrc/pybind.cpp:18-24, thirdparty/AWQ/kernels/csrc/pybind.cpp:2
 PyTorch only supplies device memory and the current stream; every computation happens in
 libkairos_mi.so.  Outputs are allocated by the caller unless the reference function returns one.
 """
+import struct
 import threading
 
 import torch
@@ -196,6 +197,189 @@ def trans_layout_c16_to_c8_awq(awq_packed, N, K):
     out = torch.empty((N, K // 2), dtype=torch.int8, device=awq_packed.device)
     _call("trans_layout_w4a8", 0, N, K, _lib.load().kmi_trans_layout_w4a8, out.data_ptr(), awq_packed.data_ptr(), N, K,
           _stream())
+    return out
+
+
+# ---- rotary positions, paged key-value cache, decode attention ------------------------------------------------------------
+KV_TILE = 32                                           # tokens of a cache tile; a page holds whole tiles
+KV_KINDS = {"f16": 0, "int8": 1, "int4": 2}
+_rope_kv_args = struct.Struct("10Q6q12i")              # kmi_rope_kv_args, kmi_kv_read_args, kmi_paged_attn_args
+_kv_read_args = struct.Struct("6Q8i")
+_paged_attn_args = struct.Struct("5Qqf9i")
+
+
+def kv_tile_bytes(head_dim, kind):
+    """Bytes of one cache tile (32 tokens of one key head, keys and values) of a kind: 'f16', 'int8' or 'int4'."""
+    if kind not in KV_KINDS:
+        raise ValueError(f"kv_tile_bytes: kind must be one of {sorted(KV_KINDS)}, got {kind!r}")
+    return _lib.check(_lib.load().kmi_kv_tile_bytes(int(head_dim), KV_KINDS[kind]))
+
+
+_CACHE_FORMS = {}                                      # tile bytes -> (head_dim, kind id); the nine sizes are distinct
+
+
+def _cache_form(cache, what):
+    """(head_dim, kind id) of a cache tensor, from the bytes of its tiles."""
+    if not _CACHE_FORMS:
+        _CACHE_FORMS.update({kv_tile_bytes(d, k): (d, i) for d in (64, 128, 256) for k, i in KV_KINDS.items()})
+    _need(cache, torch.uint8, "cache")
+    form = _CACHE_FORMS.get(cache.shape[-1]) if cache.dim() == 4 else None
+    if form is None or 0 in cache.shape:
+        raise ValueError(f"{what}: cache must be uint8 [pages, kv_heads, page_size / {KV_TILE}, kv_tile_bytes(head_dim, kind)], "
+                         f"got {tuple(cache.shape)}")
+    return form
+
+
+def _need_index(t, shape, name, what, device):
+    _need(t, torch.int32, name)
+    if tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{what}: {name} must be int32 {list(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _need_pages(page_table, batch, what, device):
+    _need(page_table, torch.int32, "page_table")
+    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1 or page_table.device != device:
+        raise ValueError(f"{what}: page_table must be int32 [{batch}, pages a sequence] on {device}, got {tuple(page_table.shape)} "
+                         f"on {page_table.device}")
+    return page_table.data_ptr(), page_table.shape[1]
+
+
+def _need_rows(x, name, what, device):
+    """fp16 [B, S, heads, D] whose heads are contiguous; returns (pointer, batch stride, token stride) in elements."""
+    if x.dtype != torch.float16:
+        raise TypeError(f"{name}: expected {torch.float16}, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}: expected a GPU tensor (the HIP library is the only compute path)")
+    if x.dim() != 4 or x.device != device:
+        raise ValueError(f"{what}: {name} must be fp16 [batch, tokens, heads, head_dim] on {device}, got {tuple(x.shape)} on {x.device}")
+    b, s, h, d = x.shape
+    sb, ss, sh, sd = x.stride()
+    if x.numel() == 0:
+        return x.data_ptr(), 0, 0
+    sb, ss = sb if b > 1 else 0, ss if s > 1 else 0
+    if (sd != 1 and d > 1) or (sh != d and h > 1) or (sb | ss) & 7 or x.data_ptr() & 15:
+        raise ValueError(f"{what}: {name}'s heads must lie behind each other, 16-byte aligned, at token and batch strides that are "
+                         f"multiples of 8 elements; got strides {tuple(x.stride())} (call .contiguous())")
+    return x.data_ptr(), sb, ss
+
+
+def _launch_on(device, name, M, N, K, fn, args):
+    """The call on the current stream of the tensors' device, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        return _call(name, M, N, K, fn, args, _stream())
+    with torch.cuda.device(device):
+        return _call(name, M, N, K, fn, args, _stream())
+
+
+def _rope_kv(what, q, k, v, start, table, interleaved, count, cache, page_table, k_out):
+    dev = k.device
+    kp, kb, kt = _need_rows(k, "k", what, dev)
+    B, S, KV, D = k.shape
+    qp = qb = qt = vp = vb = vt = H = 0
+    q_out = None
+    if q is not None:
+        qp, qb, qt = _need_rows(q, "q", what, dev)
+        H = q.shape[2]
+        if q.shape[:2] != k.shape[:2] or q.shape[3] != D or H == 0:
+            raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head_dim")
+        q_out = torch.empty((B, S, H, D), dtype=torch.float16, device=dev)
+    cp = kind = pages = tiles = pp = width = 0
+    if cache is not None:
+        cd, kind = _cache_form(cache, what)
+        vp, vb, vt = _need_rows(v, "v", what, dev)
+        if v.shape != k.shape or cd != D or cache.shape[1] != KV or cache.device != dev:
+            raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the cache {tuple(cache.shape)} "
+                             f"(head_dim {cd}) on {cache.device}")
+        pp, width = _need_pages(page_table, B, what, dev)
+        cp, pages, tiles = cache.data_ptr(), cache.shape[0], cache.shape[2]
+    tp = R = rows = 0
+    if table is not None:
+        _need(table, torch.float32, "table")
+        if table.dim() != 3 or table.shape[2] != 2 or table.device != dev:
+            raise ValueError(f"{what}: table must be fp32 [positions, rotary_dim / 2, 2] on {dev}, got {tuple(table.shape)} on {table.device}")
+        tp, rows, R = table.data_ptr(), table.shape[0], 2 * table.shape[1]
+    sp = _need_index(start, (B,), "start", what, dev)
+    np_ = 0 if count is None else _need_index(count, (B,), "count", what, dev)
+    if k.numel():
+        _launch_on(dev, "rope_kv", B * S, H + KV, D, _lib.load().kmi_rope_kv, _rope_kv_args.pack(
+            _ptr(q_out), _ptr(k_out), cp, qp, kp, vp, tp, sp, np_, pp, qb, qt, kb, kt, vb, vt,
+            B, S, H, KV, D, R, rows, 1 if interleaved else 0, kind, pages, tiles, width))
+    return q_out
+
+
+def rotary(q, k, start, table, interleaved=False, count=None):
+    """Queries and keys turned by their positions: returns (q_out, k_out), contiguous.
+
+    q fp16 [B, S, H, D], k fp16 [B, S, KV, D] (views of a fused qkv output do; D = 64, 128 or 256); token s of sequence b
+    stands at start[b] + s (int32 [B]); table fp32 [positions, R / 2, 2] of cosines and sines (kairos_amd.rotary.rotary_table),
+    R <= D a multiple of 16: the first R elements of a head turn in pairs (i, i + R/2), or (2i, 2i+1) when interleaved, the others are
+    copied.  A position outside the table gives NaN.  Tokens s >= count[b] (int32 [B]) are padding and come back as zeros."""
+    k_out = torch.empty(k.shape, dtype=torch.float16, device=k.device)
+    q_out = _rope_kv("rotary", q, k, None, start, table, interleaved, count, None, None, k_out)
+    return q_out, k_out
+
+
+def kv_append(cache, page_table, start, k, v, table=None, q=None, interleaved=False, count=None, want_k=False):
+    """Writes keys (turned by their positions when a table is given) and values of S tokens a sequence into the paged cache,
+    quantised to its kind, and turns the queries, in one launch.  Returns q_out (None without q), or (q_out, k_out) with want_k:
+    the turned keys before they were quantised.
+
+    cache uint8 [pages, KV, page_size / 32, kv_tile_bytes(D, kind)]; page_table int32 [B, pages a sequence]; q, k, v, start, table,
+    interleaved, count as in rotary().  Position t of sequence b goes to page page_table[b, t // page_size]; a token whose page is not one
+    of the cache is dropped, as is padding (s >= count[b]).  Two tokens of a call must not share a place."""
+    k_out = torch.empty(k.shape, dtype=torch.float16, device=k.device) if want_k else None
+    q_out = _rope_kv("kv_append", q, k, v, start, table, interleaved, count, cache, page_table, k_out)
+    return (q_out, k_out) if want_k else q_out
+
+
+def kv_read(cache, page_table, start, length, count=None):
+    """What the cache holds for positions start[b] .. start[b] + length - 1: (k, v) fp16 [B, length, KV, D].  Rows s >= count[b]
+    are zeros, positions without a page of this cache NaN."""
+    D, kind = _cache_form(cache, "kv_read")
+    dev, S = cache.device, int(length)
+    if S < 0 or start.dim() != 1:
+        raise ValueError(f"kv_read: start must be int32 [batch] and length >= 0, got {tuple(start.shape)} and {S}")
+    B = start.shape[0]
+    pages, KV, tiles = cache.shape[:3]
+    sp = _need_index(start, (B,), "start", "kv_read", dev)
+    np_ = 0 if count is None else _need_index(count, (B,), "count", "kv_read", dev)
+    pp, width = _need_pages(page_table, B, "kv_read", dev)
+    k = torch.empty((B, S, KV, D), dtype=torch.float16, device=dev)
+    v = torch.empty((B, S, KV, D), dtype=torch.float16, device=dev)
+    if k.numel():
+        _launch_on(dev, "kv_read", B * S, KV, D, _lib.load().kmi_kv_read, _kv_read_args.pack(
+            k.data_ptr(), v.data_ptr(), cache.data_ptr(), sp, np_, pp, B, S, KV, D, kind, pages, tiles, width))
+    return k, v
+
+
+def paged_attention(q, cache, page_table, lens, scale=None, window=0):
+    """Attention of one new token a sequence over the first lens[b] positions of its cache (its own position included):
+    fp16 like q, [B, H, D] or [B, 1, H, D].
+
+    H is a multiple of the cache's kv_heads (query head h reads key head h // (H / kv_heads)); lens int32 [B]; scale D^-0.5 by
+    default; window > 0: the last `window` positions only.  A sequence of no tokens gives zeros; one longer than its row of
+    the page table, or with a page that is not one of the cache, NaN."""
+    D, kind = _cache_form(cache, "paged_attention")
+    dev = cache.device
+    if q.dim() == 3:
+        q4 = q.unsqueeze(1)
+    elif q.dim() == 4 and q.shape[1] == 1:
+        q4 = q
+    else:
+        raise ValueError(f"paged_attention: q must be fp16 [batch, heads, head_dim] or [batch, 1, heads, head_dim], got {tuple(q.shape)}")
+    qp, qb, _ = _need_rows(q4, "q", "paged_attention", dev)
+    B, _, H, d = q4.shape
+    pages, KV, tiles = cache.shape[:3]
+    if d != D or H == 0 or H % KV:
+        raise ValueError(f"paged_attention: q {tuple(q.shape)} does not fit a cache of {KV} heads of {D}")
+    pp, width = _need_pages(page_table, B, "paged_attention", dev)
+    lp = _need_index(lens, (B,), "lens", "paged_attention", dev)
+    out = torch.empty(q.shape, dtype=torch.float16, device=dev)
+    if B:
+        _launch_on(dev, "paged_attn", B, H, D, _lib.load().kmi_paged_attn, _paged_attn_args.pack(
+            out.data_ptr(), qp, cache.data_ptr(), pp, lp, qb, D ** -0.5 if scale is None else scale,
+            B, H, KV, D, kind, pages, tiles, width, window))
     return out
 
 

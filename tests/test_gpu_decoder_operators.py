@@ -1,0 +1,466 @@
+"""GPU parity of the decoder operators behind the qkv linear (rotary positions, the paged key-value cache's writer and reader, decode
+attention over it) against the numpy oracle: rotation and cache bytes bit for bit, attention against 64 bits with a bound that counts
+the kernel's roundings."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from oracle import decoder_oracle as DO
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["f16", "int8", "int4"]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from kairos_amd import ops as _ops
+    return _ops
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def bits(t):
+    return t.cpu().numpy().view(np.uint16)
+
+
+def table_of(positions, R, base=10000.0):
+    from kairos_amd.rotary import rotary_table
+    t = rotary_table(positions, R, base, device="cpu")
+    return t.numpy(), t.cuda()
+
+
+def rotated(x, pos, table, inter):
+    """What the operator gives, bit for bit: fp32 products and sums rounded one by one, then fp16."""
+    with np.errstate(over="ignore", invalid="ignore"):
+        return DO.rotate(x, pos, table, inter, np.float32).astype(np.float16)
+
+
+def qkv_views(rng, B, S, H, KV, D):
+    qkv = rng.standard_normal((B, S, H + 2 * KV, D)).astype(np.float16)
+    t = dev(qkv)
+    return (qkv[:, :, :H], qkv[:, :, H:H + KV], qkv[:, :, H + KV:]), (t[:, :, :H], t[:, :, H:H + KV], t[:, :, H + KV:])
+
+
+# ---- rotary positions -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("D, R", [(64, 64), (64, 32), (128, 128), (128, 80), (128, 16), (256, 256), (256, 48)])
+@pytest.mark.parametrize("B, S, H, KV", [(1, 1, 4, 4), (3, 5, 7, 1), (2, 67, 8, 2)])
+def test_rotary_bit_for_bit(ops, B, S, H, KV, D, R, inter):
+    rng = np.random.default_rng(B * 1000 + S + D + R)
+    (q, k, _), (qd, kd, _) = qkv_views(rng, B, S, H, KV, D)
+    table, td = table_of(S + 40, R)
+    start = rng.integers(0, 40, B).astype(np.int32)
+    pos = start[:, None] + np.arange(S)
+    for a, b in ((qd, kd), (qd.contiguous(), kd.contiguous())):
+        qo, ko = ops.rotary(a, b, dev(start), td, interleaved=inter)
+        assert qo.is_contiguous() and qo.shape == q.shape and ko.shape == k.shape
+        assert np.array_equal(bits(qo), rotated(q, pos, table, inter).view(np.uint16))
+        assert np.array_equal(bits(ko), rotated(k, pos, table, inter).view(np.uint16))
+    # against the formula in 64 bits: half an fp16 step, and an fp32 step for each of three operations on |a| + |b|
+    exact = DO.rotate(q, pos, table, inter)
+    size = np.abs(q.astype(np.float64)).max() * 2
+    assert (np.abs(qo.cpu().numpy().astype(np.float64) - exact) <= np.abs(exact) * 2.0 ** -11 + 2.0 ** -25 + size * 3 * 2.0 ** -24).all()
+
+
+def test_rotary_keeps_lengths_and_undoes_itself(ops):
+    """A table with sines negated turns back: off by the two fp16 roundings of a pair."""
+    q = torch.randn((2, 9, 4, 128), dtype=torch.float16, device="cuda")
+    _, td = table_of(64, 128)
+    there, _ = ops.rotary(q, q, i32(3, 50), td)
+    back, _ = ops.rotary(there, there, i32(3, 50), td * torch.tensor([1.0, -1.0], device="cuda"))
+    a, b = q.float()[..., :64], q.float()[..., 64:]
+    size = torch.sqrt(a * a + b * b).repeat(1, 1, 1, 2)
+    # each turn rounds both halves of a pair by half a step (2^-11 of at most the pair's length)
+    assert ((back.float() - q.float()).abs() <= size * (2 ** 0.5 * 2.0 ** -11 + 2.0 ** -11 + 1e-6) + 2.0 ** -23).all()
+
+
+def test_rotary_padding_positions_and_empty_calls(ops):
+    q = torch.randn((3, 6, 4, 64), dtype=torch.float16, device="cuda")
+    table, td = table_of(10, 32)
+    qo, ko = ops.rotary(q, q[:, :, :2], i32(0, 7, -2), td, count=i32(4, 99, 6))
+    assert not qo[0, 4:].any() and not ko[0, 4:].any()
+    want = rotated(q.cpu().numpy()[0:1, :4], np.arange(4)[None], table, False)
+    assert np.array_equal(bits(qo[0:1, :4]), want.view(np.uint16))
+    # positions 7, 8, 9 are in the table, 10 .. 12 and -2, -1 are not: NaN in the turned elements, the others copied
+    assert torch.isfinite(qo[1, :3]).all() and torch.isnan(qo[1, 3:, :, :32]).all() and torch.isnan(qo[2, :2, :, :32]).all()
+    assert torch.equal(qo[1, 3:, :, 32:], q[1, 3:, :, 32:]) and torch.isfinite(qo[2, 2:]).all()
+    for shape in ((0, 4, 2, 64), (2, 0, 2, 64)):
+        e = torch.zeros(shape, dtype=torch.float16, device="cuda")
+        a, b = ops.rotary(e, e, torch.zeros(shape[0], dtype=torch.int32, device="cuda"), td)
+        assert a.shape == shape and b.shape == shape
+    # count 0 and below: all padding
+    a, _ = ops.rotary(q, q, i32(0, 0, 0), td, count=i32(0, -3, 1))
+    assert not a[:2].any() and not a[2, 1:].any() and a[2, 0].any()
+
+
+# ---- the cache's writer and reader ------------------------------------------------------------------------------------------
+def make_pages(rng, B, tokens, page, spare=2):
+    """int32 [B, width] over distinct pages in random order, and their number."""
+    width = -(-max(tokens, 1) // page)
+    pool = B * width + spare
+    return rng.permutation(pool)[:B * width].reshape(B, width).astype(np.int32), pool
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("S, page, starts", [(1, 32, (0, 31, 70)), (1, 96, (95, 96, 5)), (13, 32, (29, 0, 3)), (75, 64, (0, 21, 40)), (130, 160, (0, 7, 32))])
+def test_append_writes_the_oracle_s_bytes_and_read_returns_them(ops, S, page, starts, D, kind):
+    B, H, KV = 3, 4, 2
+    rng = np.random.default_rng(S + D)
+    (q, k, v), (qd, kd, vd) = qkv_views(rng, B, S, H, KV, D)
+    k[0, 0, 0] = 0; k[1, 0, 1] = 3.0; v[2, 0, 0] = -65504.0; v[0, 0, 1, ::2] = np.float16(6e-8); k[2, 0, 0, 5] = 65504.0
+    kd.copy_(dev(k)); vd.copy_(dev(v))
+    R = D // 2
+    table, td = table_of(S + 100, R)
+    pages, pool = make_pages(rng, B, max(starts) + S, page)
+    count = np.array([S, max(1, S - 3), S], np.int32)
+    start = np.array(starts, np.int32)
+    cache = rng.integers(0, 256, size=(pool, KV, page // 32, DO.tile_bytes(D, kind))).astype(np.uint8)
+    want = cache.copy()
+    pos = start[:, None] + np.arange(S)
+    kr, qr = rotated(k, pos, table, True), rotated(q, pos, table, True)
+    for b in range(B):
+        for s in range(count[b]):
+            p = pos[b, s]
+            for h in range(KV):
+                DO.put_token(want[pages[b, p // page], h, p % page // 32], p % 32, kr[b, s, h], v[b, s, h], kind)
+    cd = dev(cache)
+    qo, ko = ops.kv_append(cd, dev(pages), dev(start), kd, vd, td, q=qd, interleaved=True, count=dev(count), want_k=True)
+    got = cd.cpu().numpy()
+    assert np.array_equal(got, want), np.argwhere(got != want)[:5]         # nothing else in the pool is touched
+    for b in range(B):
+        n = count[b]
+        assert np.array_equal(bits(qo[b, :n]), qr[b, :n].view(np.uint16)) and np.array_equal(bits(ko[b, :n]), kr[b, :n].view(np.uint16))
+        assert not qo[b, n:].any() and not ko[b, n:].any()
+    rk, rv = ops.kv_read(cd, dev(pages), dev(start), S, count=dev(count))
+    for b in range(B):
+        n = count[b]
+        for x, got in ((kr, rk), (v, rv)):
+            ref = x[b, :n] if kind == "f16" else DO.to_f16(DO.values_of(*DO.quantise(x[b, :n], kind), kind, np.float32))
+            assert np.array_equal(got[b, :n].cpu().numpy().astype(np.float32), ref.astype(np.float32))
+            assert not got[b, n:].any()
+    # without queries or a table: keys as they are
+    cd = dev(cache)
+    assert ops.kv_append(cd, dev(pages), dev(start), kd, vd, count=dev(count)) is None
+    rk, _ = ops.kv_read(cd, dev(pages), dev(start), 1)
+    ref = k[:, :1] if kind == "f16" else DO.to_f16(DO.values_of(*DO.quantise(k[:, :1], kind), kind, np.float32))
+    assert np.array_equal(rk.cpu().numpy().astype(np.float32), ref.astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_pages_outside_the_cache_are_never_followed(ops, kind):
+    """Entries of -1, of the pool's size and of 2^31 - 1, and positions past the row of the page table: writes are dropped, reads give
+    NaN, neighbours are untouched."""
+    D, KV, page, pool = 64, 2, 32, 4
+    pages = i32(2, -1, pool, 2 ** 31 - 1).reshape(1, 4)
+    cache = torch.randint(0, 256, (pool, KV, 1, ops.kv_tile_bytes(D, kind)), dtype=torch.uint8, device="cuda")
+    before = cache.clone()
+    S = 150                                                        # positions 10 .. 159; the row ends at 128
+    k = torch.randn((1, S, KV, D), dtype=torch.float16, device="cuda")
+    ops.kv_append(cache, pages, i32(10), k, k)
+    changed = (cache != before).flatten(1).any(1)
+    assert changed.tolist() == [False, False, True, False]
+    rk, rv = ops.kv_read(cache, pages, i32(10), S)
+    assert torch.isfinite(rk[0, :22]).all() and torch.isnan(rk[0, 22:]).all() and torch.isnan(rv[0, 22:]).all()
+    rk, _ = ops.kv_read(cache, pages, i32(-3), 4)
+    assert torch.isnan(rk[0, :3]).all()
+    before = cache.clone()
+    ops.kv_append(cache, pages, i32(-5), k[:, :5], k[:, :5])       # positions -5 .. -1
+    assert torch.equal(cache, before)
+
+
+@pytest.mark.parametrize("kind", ["int8", "int4"])
+def test_rows_that_are_not_finite_read_as_nan(ops, kind):
+    cache = torch.zeros((1, 1, 1, ops.kv_tile_bytes(64, kind)), dtype=torch.uint8, device="cuda")
+    k = torch.randn((1, 4, 1, 64), dtype=torch.float16, device="cuda")
+    k[0, 1, 0, 3] = float("inf"); k[0, 2, 0, 60] = float("nan")
+    ops.kv_append(cache, i32(0).reshape(1, 1), i32(0), k, k)
+    rk, rv = ops.kv_read(cache, i32(0).reshape(1, 1), i32(0), 4)
+    for r in (rk, rv):
+        assert torch.isnan(r[0, 1:3]).all() and torch.isfinite(r[0, 0]).all() and torch.isfinite(r[0, 3]).all()
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------
+def attention_bound(q, k, v, scale, kind, o, mean_v, total):
+    """How far the kernel may be off: the output's rounding (2^-11), the weights' rounding to fp16 (2^-11 of each, half a subnormal
+    step of the smallest), and the scores' error -- D products added in fp32, codes with their offset (at most 1152 + 127, or
+    1024 + 15) in front of the subtraction -- which moves a weight by as much, relative.  The sums over tokens are fp32: T * 2^-24
+    of the mean size."""
+    T, D = k.shape
+    if T == 0:
+        return np.zeros(o.shape)
+    aq = np.abs(q.astype(np.float64)).sum(-1, keepdims=True)
+    kmax = np.abs(k).max()
+    big = {"f16": kmax, "int8": kmax / 100 * 1300, "int4": kmax * 1200}[kind]
+    err = scale * aq * big * (D / 8 + 8) * 2.0 ** -24 + 2.0 ** -20
+    return (np.abs(o) + mean_v) * 2.0 ** -11 + 2 * mean_v * (err + T * 2.0 ** -24) + T * 2.0 ** -25 * np.abs(v).max() / total + 2.0 ** -24
+
+
+def random_cache(rng, pool, KV, tiles, D, kind):
+    """A pool with garbage (NaN patterns among it) everywhere; tokens are put in by the caller."""
+    return rng.integers(0, 256, size=(pool, KV, tiles, DO.tile_bytes(D, kind))).astype(np.uint8)
+
+
+def filled(rng, lens, KV, D, kind, page, size=1.0):
+    """A cache written token by token by the oracle, its page table (entries behind a sequence's pages: -1), and nothing else in it
+    but garbage."""
+    need = [-(-n // page) for n in lens]
+    width = max(max(need), 1)
+    pool = sum(need) + 2
+    order = rng.permutation(pool)
+    pages = np.full((len(lens), width), -1, np.int32)
+    cache = random_cache(rng, pool, KV, page // 32, D, kind)
+    at = 0
+    for b, n in enumerate(lens):
+        pages[b, :need[b]] = order[at:at + need[b]]
+        at += need[b]
+        k, v = ((rng.standard_normal((n, KV, D)) * size).astype(np.float16) for _ in range(2))
+        for t in range(n):
+            for h in range(KV):
+                DO.put_token(cache[pages[b, t // page], h, t % page // 32], t % 32, k[t, h], v[t, h], kind)
+    return cache, pages
+
+
+def check_attention(ops, cache, pages, lens, q, KV, D, kind, window=0, scale=None, got=None):
+    H = q.shape[1]
+    G = H // KV
+    if got is None:
+        got = ops.paged_attention(dev(q), dev(cache), dev(pages), dev(np.array(lens, np.int32)), scale=scale, window=window)
+    assert got.shape == q.shape and got.dtype == torch.float16
+    got = got.cpu().numpy().astype(np.float64)
+    sc = D ** -0.5 if scale is None else scale
+    for b, n in enumerate(lens):
+        lo = max(0, n - window) if window else 0
+        for h in range(KV):
+            k, v = DO.sequence(cache, pages[b], n, h, D, kind)
+            k, v = k[lo:], v[lo:]
+            o, mean_v, total = DO.attend(q[b, h * G:(h + 1) * G], k, v, sc)
+            bound = attention_bound(q[b, h * G:(h + 1) * G], k, v, sc, kind, o, mean_v, total)
+            off = np.abs(got[b, h * G:(h + 1) * G] - o)
+            assert (off <= bound).all(), (b, h, n, float((off / np.maximum(bound, 1e-30)).max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, H, KV", [(64, 4, 4), (64, 20, 1), (128, 7, 1), (128, 8, 2), (128, 33, 1), (256, 16, 1), (256, 4, 2)])
+def test_attention_ragged_lengths(ops, D, H, KV, kind):
+    """Lengths around the tile (32), a page's end inside it, none at all, one token; query groups of 1, 4, 7, 8, 16, 20, 33."""
+    lens = [1, 0, 31, 32, 33, 100, 129]
+    rng = np.random.default_rng(D + H)
+    cache, pages = filled(rng, lens, KV, D, kind, 64)
+    q = (rng.standard_normal((len(lens), H, D)) * 2).astype(np.float16)
+    check_attention(ops, cache, pages, lens, q, KV, D, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [1, 5, 32, 64, 77, 1000])
+def test_attention_window(ops, window, kind):
+    lens = [200, 64, 3, 0]
+    rng = np.random.default_rng(window)
+    cache, pages = filled(rng, lens, 2, 64, kind, 96)
+    q = (rng.standard_normal((4, 8, 64)) * 2).astype(np.float16)
+    check_attention(ops, cache, pages, lens, q, 2, 64, kind, window=window, scale=0.2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_split_over_a_long_sequence(ops, kind):
+    """One long sequence next to short ones: its tokens are shared out over workgroups and joined."""
+    lens = [2500, 1, 40]
+    rng = np.random.default_rng(9)
+    cache, pages = filled(rng, lens, 1, 64, kind, 32)
+    q = (rng.standard_normal((3, 4, 64)) * 2).astype(np.float16)
+    check_attention(ops, cache, pages, lens, q, 1, 64, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size, qsize", [(1e-3, 1.0), (300.0, 0.05), (1.0, 30.0)])
+def test_attention_sizes_of_values_and_scores(ops, size, qsize, kind):
+    """Values far from 1 (their scales subnormal in fp16 or large), and scores so wide that one token takes all the weight."""
+    lens = [90, 33]
+    rng = np.random.default_rng(4)
+    cache, pages = filled(rng, lens, 2, 64, kind, 32, size)
+    q = (rng.standard_normal((2, 4, 64)) * qsize).astype(np.float16)
+    check_attention(ops, cache, pages, lens, q, 2, 64, kind)
+
+
+def test_attention_strided_queries_and_4d(ops):
+    rng = np.random.default_rng(2)
+    lens = [70, 45]
+    cache, pages = filled(rng, lens, 2, 64, "int8", 32)
+    qkv = (rng.standard_normal((2, 1, 8, 64)) * 2).astype(np.float16)
+    qd = dev(qkv)[:, :, :4]
+    got = ops.paged_attention(qd, dev(cache), dev(pages), i32(*lens))
+    assert got.shape == (2, 1, 4, 64) and got.is_contiguous()
+    check_attention(ops, cache, pages, lens, qkv[:, 0, :4], 2, 64, "int8", got=got[:, 0])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_errors_of_device_data_stay_in_their_sequence(ops, kind):
+    """A page that is not one of the cache and a length past the row of the page table give NaN for that sequence only."""
+    rng = np.random.default_rng(5)
+    lens = [70, 70, 70, 70]
+    cache, pages = filled(rng, lens, 2, 64, kind, 32)
+    q = rng.standard_normal((4, 4, 64)).astype(np.float16)
+    pages[1, 1] = len(cache); pages[2, 0] = -7
+    given = np.array([70, 70, 70, 97], np.int32)                    # the row holds 96
+    got = ops.paged_attention(dev(q), dev(cache), dev(pages), dev(given))
+    assert torch.isnan(got[1:]).all() and torch.isfinite(got[0]).all()
+    check_attention(ops, cache, pages[:1], lens[:1], q[:1], 2, 64, kind, got=got[:1])
+    neg = ops.paged_attention(dev(q), dev(cache), dev(pages), i32(-1, 0, -2 ** 31, 0))
+    assert not neg.any()
+    e = ops.paged_attention(torch.zeros((0, 4, 64), dtype=torch.float16, device="cuda"), dev(cache), dev(pages[:0]), dev(given[:0]))
+    assert e.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_cache_beyond_32_bit_offsets(ops, kind):
+    """Pages whose bytes lie past 4 GiB, written, read and attended to as those at the start."""
+    D, KV, page = 256, 8, 256
+    per = KV * (page // 32) * ops.kv_tile_bytes(D, kind)
+    pool = (5 << 30) // per
+    cache = torch.empty((pool, KV, page // 32, ops.kv_tile_bytes(D, kind)), dtype=torch.uint8, device="cuda")
+    S = 300
+    k, v = (torch.randn((1, S, KV, D), dtype=torch.float16, device="cuda") for _ in range(2))
+    q = torch.randn((1, 16, D), dtype=torch.float16, device="cuda")
+    near, far = i32(0, 1).reshape(1, 2), i32(pool - 1, pool - 2).reshape(1, 2)
+    outs = []
+    for pages in (near, far):
+        ops.kv_append(cache, pages, i32(0), k, v)
+        outs.append(ops.kv_read(cache, pages, i32(0), S) + (ops.paged_attention(q, cache, pages, i32(S)),))
+    for a, b in zip(*outs):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    del cache
+
+
+# ---- together, streams, graphs -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_generation_step_by_step(ops, kind):
+    """Prefill of unequal prompts (padded batch), then tokens one by one: rotate, append and attend as a decoder layer does, against the
+    attention of the oracle over everything the cache holds so far."""
+    from kairos.kv_cache import PagedKVCache
+    from kairos.rotary import rotary_table
+    B, H, KV, D, page = 2, 8, 2, 64, 32
+    rng = np.random.default_rng(1)
+    count = np.array([37, 20], np.int32)
+    S = int(count.max())
+    table = rotary_table(128, D, 500000.0, {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 64})
+    c = PagedKVCache(8, KV, D, kind, page)
+    pages, _ = make_pages(rng, B, 96, page)
+    _, (q, k, v) = qkv_views(rng, B, S, H, KV, D)
+    c.append(dev(pages), i32(0, 0), k, v, table, q=q, count=dev(count))
+    lens = count.copy()
+    for step in range(4):
+        _, (q, k, v) = qkv_views(rng, B, 1, H, KV, D)
+        qo = c.append(dev(pages), dev(lens), k, v, table, q=q)
+        want_q = rotated(q.cpu().numpy(), lens[:, None], table.cpu().numpy(), False)
+        assert np.array_equal(bits(qo), want_q.view(np.uint16))
+        lens = lens + 1
+        out = c.attend(qo, dev(pages), dev(lens))
+        check_attention(ops, c.data.cpu().numpy(), pages, list(lens), want_q[:, 0], KV, D, kind, got=out[:, 0])
+        rk, _ = c.read(dev(pages), dev(lens - 1), 1)
+        key = rotated(k.cpu().numpy(), (lens - 1)[:, None], table.cpu().numpy(), False)
+        ref = key if kind == "f16" else DO.to_f16(DO.values_of(*DO.quantise(key, kind), kind, np.float32))
+        assert np.array_equal(rk.cpu().numpy().astype(np.float32), ref.astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_step_replays_as_eager(ops, kind):
+    """One decode step (append + attend, position on the device) captured once and replayed with the program's own eager work in
+    between; every replay equals the eager step bit for bit, also where two graphs replay in turn on one stream."""
+    from kairos.rotary import rotary_table
+    B, H, KV, D, page = 3, 8, 2, 128, 64
+    table = rotary_table(2048, D)
+    pages = torch.randperm(B * 20, device="cuda")[:B * 20].to(torch.int32).reshape(B, 20).contiguous()
+    shape = (B * 20, KV, page // 32, ops.kv_tile_bytes(D, kind))
+    seed = torch.randn((B, 1000, KV, D), dtype=torch.float16, device="cuda")
+    caches = [torch.zeros(shape, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    for c in caches:
+        ops.kv_append(c, pages, i32(0, 0, 0), seed, seed)
+    qkv = torch.randn((B, 1, H + 2 * KV, D), dtype=torch.float16, device="cuda")
+    pos = i32(1000, 40, 0)
+
+    def step(cache):
+        q = ops.kv_append(cache, pages, pos, qkv[:, :, H:H + KV], qkv[:, :, H + KV:], table, q=qkv[:, :, :H])
+        return ops.paged_attention(q, cache, pages, pos + 1)
+
+    side = torch.cuda.Stream()
+    scratch = ops.Scratch()
+    graphs, outs = [], []
+    side.wait_stream(torch.cuda.current_stream())
+    for c in caches[:2]:
+        with torch.cuda.stream(side), scratch:
+            step(c)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with scratch, torch.cuda.graph(g, stream=side):
+            outs.append(step(c))
+        graphs.append(g)
+    for i in range(4):
+        qkv.copy_(torch.randn(qkv.shape, dtype=torch.float16, device="cuda"))
+        for g in graphs:
+            g.replay()
+        want = step(caches[2])
+        torch.cuda.synchronize()
+        for o, c in zip(outs, caches):
+            assert torch.equal(o.view(torch.int16), want.view(torch.int16)), i
+            assert torch.equal(c, caches[2])
+        pos.add_(1)
+
+
+def test_streams_of_their_own(ops):
+    """Calls on two streams at once, each ordered behind its inputs: the results of one stream alone."""
+    D, KV, H, page = 128, 4, 16, 64
+    cache = torch.randn((80, KV, page // 32, ops.kv_tile_bytes(D, "f16") // 2), device="cuda").half().view(torch.uint8)
+    pages = torch.arange(80, dtype=torch.int32, device="cuda").reshape(2, 40)
+    qs = [torch.randn((2, H, D), dtype=torch.float16, device="cuda") for _ in range(8)]
+    lens = i32(2500, 77)
+    want = [ops.paged_attention(q, cache, pages, lens) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * len(qs)
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = ops.paged_attention(q, cache, pages, lens)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------------------
+def test_refusals(ops):
+    q = torch.zeros((2, 3, 4, 64), dtype=torch.float16, device="cuda")
+    k = torch.zeros((2, 3, 2, 64), dtype=torch.float16, device="cuda")
+    start, pages = i32(0, 0), i32(0, 1).reshape(2, 1)
+    table = torch.zeros((8, 32, 2), device="cuda")
+    cache = torch.zeros((2, 2, 1, ops.kv_tile_bytes(64, "int8")), dtype=torch.uint8, device="cuda")
+    cases = [
+        (lambda: ops.rotary(q.float(), k, start, table), TypeError), (lambda: ops.rotary(q, k, start.long(), table), TypeError),
+        (lambda: ops.rotary(q, k, start[:1], table), ValueError), (lambda: ops.rotary(q[:1], k, start, table), ValueError),
+        (lambda: ops.rotary(q, k, start, table.half()), TypeError), (lambda: ops.rotary(q, k, start, table[..., :1]), ValueError),
+        (lambda: ops.rotary(q, k, start, table[:, :30].contiguous()), Exception), (lambda: ops.rotary(q.transpose(2, 3), k, start, table), ValueError),
+        (lambda: ops.rotary(q[..., 4:36], k[..., 4:36], start, table), ValueError), (lambda: ops.rotary(q, k, start, table, count=i32(1)), ValueError),
+        (lambda: ops.rotary(q[..., :32].contiguous(), k[..., :32].contiguous(), start, table), Exception),
+        (lambda: ops.kv_append(cache, pages, start, k[:, :, :1], k[:, :, :1]), ValueError), (lambda: ops.kv_append(cache, pages[:1], start, k, k), ValueError),
+        (lambda: ops.kv_append(cache, pages.long(), start, k, k), TypeError), (lambda: ops.kv_append(cache[..., :100].contiguous(), pages, start, k, k), ValueError),
+        (lambda: ops.kv_append(cache, pages, start, k, k[:, :2]), ValueError), (lambda: ops.kv_append(cache.to(torch.int8), pages, start, k, k), TypeError),
+        (lambda: ops.kv_append(cache.transpose(0, 1), pages, start, k, k), ValueError), (lambda: ops.kv_append(cache, pages, start, k.cpu(), k), ValueError),
+        (lambda: ops.kv_read(cache, pages, start, -1), ValueError), (lambda: ops.kv_read(cache, pages, start[:1], 3), ValueError),
+        (lambda: ops.kv_read(cache, pages, start, 3, count=start.float()), TypeError),
+        (lambda: ops.paged_attention(q[:, :2], cache, pages, start), ValueError), (lambda: ops.paged_attention(q[:, 0, :3], cache, pages, start), ValueError),
+        (lambda: ops.paged_attention(q[:, 0], cache, pages, start, scale=0.0), Exception), (lambda: ops.paged_attention(q[:, 0], cache, pages, start, window=-1), Exception),
+        (lambda: ops.paged_attention(q[:, 0], cache, pages, i32(1)), ValueError), (lambda: ops.paged_attention(q[:, 0].cpu(), cache, pages, start), ValueError),
+    ]
+    for i, (call, err) in enumerate(cases):
+        with pytest.raises(err):
+            call()
+            print("accepted", i)
