@@ -205,7 +205,7 @@ KV_TILE = 32                                           # tokens of a cache tile;
 KV_KINDS = {"f16": 0, "int8": 1, "int4": 2}
 _rope_kv_args = struct.Struct("10Q6q12i")              # kmi_rope_kv_args, kmi_kv_read_args, kmi_paged_attn_args
 _kv_read_args = struct.Struct("6Q8i")
-_paged_attn_args = struct.Struct("5Qqf9i")
+_paged_attn_args = struct.Struct("7Qqf9i")
 
 
 def kv_tile_bytes(head_dim, kind):
@@ -377,9 +377,19 @@ def paged_attention(q, cache, page_table, lens, scale=None, window=0):
     lp = _need_index(lens, (B,), "lens", "paged_attention", dev)
     out = torch.empty(q.shape, dtype=torch.float16, device=dev)
     if B:
-        _launch_on(dev, "paged_attn", B, H, D, _lib.load().kmi_paged_attn, _paged_attn_args.pack(
-            out.data_ptr(), qp, cache.data_ptr(), pp, lp, qb, D ** -0.5 if scale is None else scale,
-            B, H, KV, D, kind, pages, tiles, width, window))
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                return paged_attention(q, cache, page_table, lens, scale, window)
+        st = _stream()
+        ws = gemv_workspace_for(dev, st)
+        try:
+            _call("paged_attn", B, H, D, _lib.load().kmi_paged_attn, _paged_attn_args.pack(
+                out.data_ptr(), qp, cache.data_ptr(), pp, lp, ws.data_ptr(), ws.numel(), qb, D ** -0.5 if scale is None else scale,
+                B, H, KV, D, kind, pages, tiles, width, window), st)
+        except _lib.KairosMiError as e:
+            if e.code == -6:               # the runtime rejected a launch: leave the counters in a known state
+                _lib.load().kmi_gemv_ws_reset(ws.data_ptr(), ws.numel(), st)
+            raise
     return out
 
 

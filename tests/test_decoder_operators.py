@@ -133,7 +133,7 @@ ROPE = dict(q_out=16, k_out=16, cache=16, q=16, k=16, v=16, table=16, start=16, 
             kind=0, num_pages=4, page_tiles=1, max_pages=4)
 READ = dict(k_out=16, v_out=16, cache=16, start=16, count=0, page_table=16, B=1, S=1, KV=2, D=64, kind=0, num_pages=4, page_tiles=1,
             max_pages=4)
-ATTN = dict(out=16, q=16, cache=16, page_table=16, lens=16, q_batch=0, scale=0.125, B=1, H=4, KV=2, D=64, kind=0, num_pages=4,
+ATTN = dict(out=16, q=16, cache=16, page_table=16, lens=16, workspace=16, workspace_bytes=1 << 30, q_batch=0, scale=0.125, B=1, H=4, KV=2, D=64, kind=0, num_pages=4,
             page_tiles=1, max_pages=4, window=0)
 
 
@@ -172,7 +172,8 @@ def test_kv_read_refusals(lib, change, code):
 @pytest.mark.parametrize("change, code", [
     (dict(out=0), -1), (dict(q=0), -1), (dict(lens=0), -1), (dict(cache=0), -1), (dict(page_table=0), -1), (dict(out=8), -5), (dict(q=8), -5),
     (dict(q_batch=4), -5), (dict(H=5), -2), (dict(H=0), -2), (dict(KV=3), -2), (dict(D=80), -2), (dict(kind=9), -2), (dict(window=-1), -2),
-    (dict(scale=0.0), -2), (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(B=0), 0),
+    (dict(scale=0.0), -2), (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(workspace=0), -2),
+    (dict(workspace_bytes=1 << 16), -2), (dict(workspace=8), -5), (dict(B=65535, KV=2, H=4, max_pages=1 << 20), -2), (dict(B=0), 0),
 ])
 def test_paged_attn_refusals(lib, change, code):
     from kairos_amd import ops
@@ -185,7 +186,7 @@ def test_structs_have_the_header_s_size():
     from kairos_amd import ops
     assert ops._rope_kv_args.size == 10 * 8 + 6 * 8 + 12 * 4
     assert ops._kv_read_args.size == 6 * 8 + 8 * 4
-    assert ops._paged_attn_args.size == 5 * 8 + 8 + 4 + 9 * 4
+    assert ops._paged_attn_args.size == 7 * 8 + 8 + 4 + 9 * 4
 
 
 def test_python_layer_refuses_cpu_tensors_and_wrong_forms(lib):
