@@ -6,17 +6,44 @@
 //   O^T [d x head]    += V^T P^T    (16x16x32 MFMA, a step's 32 tokens deep)
 // The cache's tile order makes the result registers of the first product, lane (head, g) = tokens 8 g .. 8 g + 7, the operand
 // registers of the second: nothing passes through LDS or between lanes but the maximum over the four lane groups.
-// Codes enter the products as fp16 integers.  Keys go in as 1024 + u (one byte permute or mask, no subtraction); the offset
-// times the sum of q is taken off in fp32, where the score's factor is applied.  Values go in as small signed integers; the
-// token's scale multiplies p, relative to a running power of two so that p stays normal in fp16, and the offsets of the int4
-// kind add up to one scalar a head.
+// Codes enter the products masked where they stand, as fp16 subnormals (the MFMA takes them exactly): one instruction for two.  A key's
+// factors meet its score in fp32, with the sum of q for the offset.  A value's scale multiplies p, relative to a running power of two
+// so that p stays normal in fp16; the middle of the codes is taken off the sums at the end by the sum of the same rounded weights (one
+// more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to one scalar a head.
 #include "kv_parts.h"
 
-#ifndef KMI_PA_RUNS
-#define KMI_PA_RUNS 512
+#ifndef PA_RUNS_EXPR
+#define PA_RUNS_EXPR 256
 #endif
+#ifndef PA_QUARTETS
+#define PA_QUARTETS 2
+#endif
+#ifndef PA_BOUND
+#define PA_BOUND 1
+#endif
+#ifndef PA_DEPTH
+#define PA_DEPTH 1
+#endif
+#ifndef PA_SCHED
+#define PA_SCHED __builtin_amdgcn_sched_barrier(0)
+#endif
+#ifndef PA_LDS
+#define PA_LDS 0
+#endif
+#ifndef PA_R64
+#define PA_R64 4
+#endif
+#ifndef PA_R128
+#define PA_R128 3
+#endif
+// Workgroups (four waves) that a CU holds at once: what the registers of the accumulators, the operand of q and a tile in flight leave.
+static constexpr int pa_resident(int D) { return D == 64 ? PA_R64 : D == 128 ? PA_R128 : 2; }
 #ifndef KMI_PA_MIN_QUOTA
 #define KMI_PA_MIN_QUOTA 8
+#endif
+
+#ifndef PA_TASK_COST
+#define PA_TASK_COST 6
 #endif
 
 static constexpr float PA_NEG = -1e30f;       // running maximum before the first token: finite, so differences stay numbers
@@ -35,210 +62,287 @@ __device__ __forceinline__ float over_groups(float v, F f) {
 __device__ __forceinline__ float group_max(float v) { return over_groups(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float group_sum(float v) { return over_groups(v, [](float a, float b) { return a + b; }); }
 
-// Eight halves of unit u (0 .. n - 1) of a 16-byte key chunk: the element itself, or 1024 + code.
+// Eight halves of unit u (0 .. n - 1) of a 16-byte key chunk, element e times key_weight(e): the element itself, or its code u as
+// the subnormal u * 2^-24 (int4 elements 2, 3, 6, 7, masked where they stand: u * 2^-20, and q / 16 makes up for it).
 template <int KIND>
 __device__ __forceinline__ h8_t key_unit(const u4_t& c, int u) {
-    if constexpr (KIND == KMI_KV_F16) {
-        return __builtin_bit_cast(h8_t, c);
-    } else if constexpr (KIND == KMI_KV_INT8) {
-        u4_t o;
-        o[0] = __builtin_amdgcn_perm(0x64646464u, c[2 * u], 0x04010400u);
-        o[1] = __builtin_amdgcn_perm(0x64646464u, c[2 * u], 0x04030402u);
-        o[2] = __builtin_amdgcn_perm(0x64646464u, c[2 * u + 1], 0x04010400u);
-        o[3] = __builtin_amdgcn_perm(0x64646464u, c[2 * u + 1], 0x04030402u);
-        return __builtin_bit_cast(h8_t, o);
-    } else {
-        u4_t o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = ((c[u] >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
-        return __builtin_bit_cast(h8_t, o);
+    u4_t o = c;
+    if constexpr (KIND == KMI_KV_INT8) {
+        o[0] = __builtin_amdgcn_perm(0u, c[2 * u], 0x0C010C00u);
+        o[1] = __builtin_amdgcn_perm(0u, c[2 * u], 0x0C030C02u);
+        o[2] = __builtin_amdgcn_perm(0u, c[2 * u + 1], 0x0C010C00u);
+        o[3] = __builtin_amdgcn_perm(0u, c[2 * u + 1], 0x0C030C02u);
+    } else if constexpr (KIND == KMI_KV_INT4) {
+        const uint32_t w = c[u], w8 = w >> 8;
+        o[0] = w & 0x000F000Fu;
+        o[1] = w & 0x00F000F0u;
+        o[2] = w8 & 0x000F000Fu;
+        o[3] = w8 & 0x00F000F0u;
     }
+    return __builtin_bit_cast(h8_t, o);
 }
 
-// Value a (0 .. n - 1) of the eight tokens of a 16-byte value chunk: the element, or code - 128 / code - 8.
+// Value a (0 .. n - 1) of the eight tokens of a 16-byte value chunk: the element, or its code u as the subnormal u * 2^-24,
+// int4 with odd a u * 2^-20.
 template <int KIND>
 __device__ __forceinline__ h8_t value_unit(const u4_t& c, int a) {
-    if constexpr (KIND == KMI_KV_F16) {
-        return __builtin_bit_cast(h8_t, c);
-    } else {
-        u4_t o;
+    u4_t o = c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h2_t v;
-            if constexpr (KIND == KMI_KV_INT8) {
-                const h2_t off = {(half_t)1152.0f, (half_t)1152.0f};
-                v = as_h2(__builtin_amdgcn_perm(0x64646464u, c[i], a ? 0x04030401u : 0x04020400u)) - off;
-            } else {
-                const uint32_t w = a & 2 ? c[i] >> 8 : c[i];
-                const h2_t off = {(half_t)1032.0f, (half_t)1032.0f}, off16 = {(half_t)-72.0f, (half_t)-72.0f};
-                const h2_t sixteenth = {(half_t)0.0625f, (half_t)0.0625f};
-                v = a & 1 ? pk_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, off16)
-                          : as_h2((w & 0x000F000Fu) | 0x64006400u) - off;
-            }
-            o[i] = as_u32(v);
-        }
-        return __builtin_bit_cast(h8_t, o);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (KIND == KMI_KV_INT8) o[i] = a ? __builtin_amdgcn_perm(0u, c[i], 0x0C030C01u) : c[i] & 0x00FF00FFu;
+        if constexpr (KIND == KMI_KV_INT4) o[i] = (a & 2 ? c[i] >> 8 : c[i]) & (a & 1 ? 0x00F000F0u : 0x000F000Fu);
     }
+    return __builtin_bit_cast(h8_t, o);
 }
 
-// One wave's share of one head's tokens.
-template <int D, int KIND>
+// One wave's share of one head's tokens.  PACK = 2 (at most 8 query heads): columns 0-7 of the product are the heads on the tokens of
+// the tile's half h = 0, columns 8-15 the same heads on half 1, each with a running maximum of its own: q stands twice in
+// the operand, zero in the other half's columns, and every lane has four scores a tile instead of eight.
+template <int D, int KIND, int PACK>
 struct PaWave {
     static constexpr int n = kv_per_word(KIND), CH = D / 16 / n, KSTEPS = D / 32, OT = D / 16, NF = kv_factors(KIND);
     static constexpr int TILE_BYTES = kv_tile_bytes(D, KIND), PART = kv_part_bytes(D, KIND);
-    h8_t q[KSTEPS];             // lane (head, g): q[32 kk + 8 g ..]
-    f4_t acc[OT];               // lane (head, g): tile T = n c + a, rows dl = 4 g + r, d = 16 n c + n dl + a
-    float m, l, zsum;           // running maximum (raw scores; the head's), this lane's share of the sums of p and p * offset
-    float ref;                  // power of two that the value scales are relative to
-    float qsum;
+    static constexpr int NS = 8 / PACK;                        // scores a lane holds of a tile
+    static constexpr bool CODES = KIND != KMI_KV_F16;
+    typedef _Float16 fac_t __attribute__((ext_vector_type(NS)));
+    h8_t q[PACK][KSTEPS];       // lane (column, g): q[32 kk + 8 g ..]
+    f4_t acc[OT];               // lane (column, g): tile T = n c + a, rows dl = 4 g + r, d = 16 n c + n dl + a
+    f4_t psum;                  // sum of the weights that entered acc (every row the same)
+    float m;                    // the column's reference: weights are p = 2^(x - m), x = score * scale * log2(e)
+    float l, zsum;              // this lane's share of the sums of p and of p * offset
+    float c, qc;                // scale * log2(e), for codes times 2^24 (their unit); sum of q, times scale * log2(e)
 
-    __device__ __forceinline__ void start(const half_t* qrow, bool used, int g) {
+    __device__ __forceinline__ void start(const half_t* qrow, bool used, int col, int g, float scale) {
         float s = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) {
-            q[kk] = used ? *reinterpret_cast<const h8_t*>(qrow + 32 * kk + 8 * g) : h8_t{};
+            h8_t x = used ? *reinterpret_cast<const h8_t*>(qrow + 32 * kk + 8 * g) : h8_t{};
+            if constexpr (CODES) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += (float)q[kk][e];
+                for (int e = 0; e < 8; ++e) s += (float)x[e];
+            }
+            if constexpr (KIND == KMI_KV_INT4) {
+                const h8_t weight = {1.0f, 1.0f, 0.0625f, 0.0625f, 1.0f, 1.0f, 0.0625f, 0.0625f};
+                x = x * weight;
+            }
+            if constexpr (PACK == 1) {
+                q[0][kk] = x;
+            } else {
+                q[0][kk] = col < 8 ? x : h8_t{};
+                q[1][kk] = col < 8 ? h8_t{} : x;
+            }
         }
-        qsum = KIND == KMI_KV_F16 ? 0.0f : group_sum(s);
+        c = CODES ? scale * 0x1p24f : scale;
+        qc = CODES ? group_sum(s) * scale : 0.0f;
 #pragma unroll
         for (int t = 0; t < OT; ++t) acc[t] = f4_t{};
-        m = PA_NEG; l = 0.0f; zsum = 0.0f; ref = 0x1p-24f;
+        psum = f4_t{};
+        m = PA_NEG; l = 0.0f; zsum = 0.0f;
     }
 
     struct Factors {
-        h8_t f[NF ? NF : 1];
+        fac_t f[NF ? NF : 1];
     };
     struct Tile {
         u4_t k[CH], v[CH];
         Factors f;
     };
     struct Scores {
-        float s[8];
+        float s[NS];
     };
+    // The first of the lane's NS tokens in a tile.
+    static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
+
     __device__ __forceinline__ void load_keys(Tile& t, const char* tile, int lane) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) t.k[i] = *reinterpret_cast<const u4_t*>(tile + i * 1024 + lane * 16);
 #pragma unroll
-        for (int i = 0; i < NF; ++i) t.f.f[i] = *reinterpret_cast<const h8_t*>(tile + 2 * PART + 64 * i + (lane >> 4) * 16);
+        for (int i = 0; i < NF; ++i) t.f.f[i] = *reinterpret_cast<const fac_t*>(tile + 2 * PART + 64 * i + 2 * first_token(lane));
     }
     __device__ __forceinline__ void load_values(Tile& t, const char* tile, int lane) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) t.v[i] = *reinterpret_cast<const u4_t*>(tile + PART + i * 1024 + lane * 16);
     }
 
-    // Raw scores of the lane's tokens 8 g + j and head.
-    __device__ __forceinline__ Scores scores(const Tile& t) const {
-        f4_t s4[2];
+    // Raw scores of the lane's tokens and column.
+    __device__ __forceinline__ Scores scores(const Tile& t, int lane) const {
+        f4_t s4[2] = {f4_t{}, f4_t{}};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            s4[h] = f4_t{};
+        for (int kk = 0; kk < KSTEPS; ++kk) {
 #pragma unroll
-            for (int kk = 0; kk < KSTEPS; ++kk) {
+            for (int h = 0; h < 2; ++h) {
                 const int unit = h * KSTEPS + kk;
-                s4[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_unit<KIND>(t.k[unit / n], unit % n), q[kk], s4[h], 0, 0, 0);
+                s4[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_unit<KIND>(t.k[unit / n], unit % n), q[PACK == 2 ? h : 0][kk], s4[h], 0, 0, 0);
             }
+        }
+        if constexpr (PACK == 2) {                             // a choice, no sum: zero times a masked token's contents may be NaN
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s4[0][r] = lane & 8 ? s4[1][r] : s4[0][r];
         }
         Scores o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            o.s[j] = s4[j >> 2][j & 3];
-            if constexpr (KIND == KMI_KV_INT8) o.s[j] = (o.s[j] - 1152.0f * qsum) * (float)t.f.f[0][j];
-            if constexpr (KIND == KMI_KV_INT4) o.s[j] = (o.s[j] - 1024.0f * qsum) * (float)t.f.f[0][j] + qsum * (float)t.f.f[1][j];
-        }
+        for (int j = 0; j < NS; ++j) o.s[j] = s4[j >> 2][j & 3];
         return o;
     }
-    // The weights p (fp16 operand) from the scores, and the running maximum, sums and accumulators brought to them; v: the
-    // tile's values, fac: its factors.  tok0 = the lane's first token, [lo, hi) the tokens that count, whole = the tile lies
-    // inside.  bad: no page of this cache.  c = scale * log2(e).
-    __device__ __forceinline__ h8_t weights(Scores& sc, u4_t (&val)[CH], Factors& fac, int tok0, int lo, int hi, bool whole, bool bad, float c) {
-        float (&s)[8] = sc.s;
-        if (bad) {
+    // x - less of a product's result: the score in powers of two.
+    __device__ __forceinline__ float exponent(float s, const Factors& fac, int j, float less) const {
+        if constexpr (KIND == KMI_KV_F16) return __builtin_fmaf(s, c, -less);
+        if constexpr (KIND == KMI_KV_INT8) return __builtin_fmaf(__builtin_fmaf(s, c, -128.0f * qc), (float)fac.f[0][j], -less);
+        return __builtin_fmaf(s * c, (float)fac.f[0][j], __builtin_fmaf(qc, (float)fac.f[1][j], -less));
+    }
+    // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
+    // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (to the largest x plus
+    // the logarithm of the largest value scale) only where a weight would pass 2^10 or p 2^40, which is seldom after a wave's
+    // first tile: no reduction over lanes otherwise.  val: the tile's values, fac: its factors, tok: its first token, [lo, hi)
+    // the tokens that count, whole: the tile lies inside, bad: no page of this cache.
+    __device__ __forceinline__ h8_t weights(const Scores& sc, u4_t (&val)[CH], Factors& fac, int tok, int lo, int hi, bool whole, bool bad,
+                                            int lane) {
+        float vs[NS], y[NS], p[NS], wt[NS];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = __builtin_nanf("");
+        for (int j = 0; j < NS; ++j) {
+            vs[j] = CODES ? (float)fac.f[NF / 2][j] : 1.0f;
+            y[j] = exponent(sc.s[j], fac, j, m);
         }
-        float vs[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vs[j] = KIND == KMI_KV_F16 ? 1.0f : (float)fac.f[NF / 2][j];
         if (!whole) {
             // tokens outside: no weight, and nothing that stands in their place may reach a product
-            u4_t keep;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) keep[i] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool in = tok0 + j >= lo && tok0 + j < hi;
-                s[j] = in ? s[j] : -__builtin_inff();
+            for (int j = 0; j < NS; ++j) {
+                const int t = tok + first_token(lane) + j;
+                const bool in = t >= lo && t < hi;
+                y[j] = in ? y[j] : -__builtin_inff();
                 vs[j] = in ? vs[j] : 0.0f;
                 if constexpr (KIND == KMI_KV_INT4) fac.f[3][j] = in ? fac.f[3][j] : (half_t)0.0f;
-                keep[j >> 1] |= in ? 0xFFFFu << (16 * (j & 1)) : 0u;
             }
-            if constexpr (KIND == KMI_KV_F16) {
+            if constexpr (!CODES) {
+                u4_t keep = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int t = tok + 8 * (lane >> 4) + j;
+                    keep[j >> 1] |= t >= lo && t < hi ? 0xFFFFu << (16 * (j & 1)) : 0u;
+                }
 #pragma unroll
                 for (int i = 0; i < CH; ++i) val[i] &= keep;
             }
         }
-        float top = s[0];
+        if (bad) {
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
-        top = group_max(top);
-        float vtop = 0.0f;
-        if constexpr (KIND != KMI_KV_F16) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) vtop = fmaxf(vtop, vs[j]);
-            vtop = group_max(vtop);
+            for (int j = 0; j < NS; ++j) y[j] = __builtin_nanf("");
         }
-        if (__any(top > m) || vtop > ref) {
-            const float m2 = fmaxf(m, top);
-            float a = __builtin_amdgcn_exp2f((m - m2) * c);
-            l *= a; zsum *= a;
-            m = m2;
-            if (KIND != KMI_KV_F16 && vtop > ref) {                // the next power of two: products with it are exact
-                const float r2 = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, vtop) + 0x7FFFFFu) & 0x7F800000u);
-                a *= ref / r2;
-                ref = r2;
+        float wtop = 0.0f, ytop = PA_NEG;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(y[j]);
+            wt[j] = CODES ? p[j] * vs[j] : p[j];
+            wtop = fmaxf(wtop, wt[j]);
+            if constexpr (CODES) ytop = fmaxf(ytop, y[j]);
+        }
+        if (__any(wtop > 1024.0f || ytop > 40.0f)) {
+            float top = -__builtin_inff(), vtop = 0x1p-24f;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                // from the products again: y is what m left of x
+                y[j] = y[j] == -__builtin_inff() ? y[j] : exponent(sc.s[j], fac, j, 0.0f);
+                top = fmaxf(top, y[j]);
+                vtop = fmaxf(vtop, vs[j]);
             }
+            top = group_max(top);
+            if constexpr (CODES) top += __builtin_amdgcn_logf(group_max(vtop));
+            const float m2 = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            l *= a; zsum *= a;
+            if constexpr (CODES) psum = psum * a;
 #pragma unroll
             for (int i = 0; i < OT; ++i) acc[i] = acc[i] * a;
-        }
-        const float inv = 1.0f / ref, mc = m * c;
-        h8_t pf;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -mc));
-            l += p;
-            if constexpr (KIND == KMI_KV_INT4) zsum += p * ((float)fac.f[3][j] + 8.0f * vs[j]);
-            pf[j] = (half_t)(KIND == KMI_KV_F16 ? p : p * (vs[j] * inv));
+            for (int j = 0; j < NS; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(y[j] - m);
+                wt[j] = CODES ? p[j] * vs[j] : p[j];
+            }
+        }
+        h8_t pf = {};
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            l += p[j];
+            if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(8.0f, vs[j], (float)fac.f[3][j]), zsum);
+            pf[j] = (half_t)wt[j];
+        }
+        if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
+            const u4_t w = __builtin_bit_cast(u4_t, pf);
+            const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
+            pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
         }
         return pf;
     }
-    // The sums as they stand: value scales' unit and the offsets' sum applied.
-    __device__ __forceinline__ void unscale() {
-        if constexpr (KIND == KMI_KV_F16) return;
-#pragma unroll
-        for (int T = 0; T < OT; ++T) acc[T] = acc[T] * ref + zsum;
-    }
-    static __device__ __forceinline__ int d_of(int T, int dl) { return 16 * n * (T / n) + n * dl + T % n; }
     __device__ __forceinline__ void add(const u4_t (&val)[CH], const h8_t& pf) {
 #pragma unroll
         for (int T = 0; T < OT; ++T)
             acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(val[T / n], T % n), pf, acc[T], 0, 0, 0);
+        if constexpr (CODES) {
+            const half_t one = (half_t)1.0f;
+            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, pf, psum, 0, 0, 0);
+        }
     }
+    // The sums as they stand: over the lane groups, and for codes the units, the codes' middle (taken off with the very
+    // weights that entered the products, so their rounding cancels) and the offsets.  PACK 2: the two halves joined, in both.
+    __device__ __forceinline__ void finish() {
+        l = group_sum(l);
+        if constexpr (CODES) {
+            if constexpr (KIND == KMI_KV_INT4) zsum = group_sum(zsum);
+            const float off = KIND == KMI_KV_INT8 ? 128.0f * psum[0] : 8.0f * psum[0];
+#pragma unroll
+            for (int T = 0; T < OT; ++T) {
+                const float unit = KIND == KMI_KV_INT4 && (T & 1) ? 0x1p20f : 0x1p24f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[T][r] = __builtin_fmaf(acc[T][r], unit, -off) + zsum;
+            }
+        }
+        if constexpr (PACK == 2) {
+            const float m2 = fmaxf(m, other_half(m)), a = __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            l *= a;
+            l += other_half(l);
+#pragma unroll
+            for (int T = 0; T < OT; ++T)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float x = acc[T][r] * a;
+                    acc[T][r] = x + other_half(x);
+                }
+        }
+    }
+    static __device__ __forceinline__ float other_half(float v) {          // row_ror 8: column c ^ 8 of the same lane group
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
+    }
+    static __device__ __forceinline__ int d_of(int T, int dl) { return 16 * n * (T / n) + n * dl + T % n; }
 };
 
-// Work is shared out by tiles: the tiles of all tasks (sequence, 16 query heads of a key head) stand in a row, sequence by
-// sequence, and workgroup w takes the run [w * quota, (w + 1) * quota) of them, whatever the lengths are -- the lengths are on the
-// device, so every workgroup adds them up itself.  A task that lies in one run is finished there; one cut by run borders leaves a
-// partial sum per workgroup (at most two each: the task that a run begins in the middle of, and the one that it ends in the
-// middle of), and whichever workgroup of a task arrives last joins them in order.
+// Work is shared out by tiles.  The lengths are on the device, so every workgroup works the shares out itself, the same way:
+//   quota q = tiles of all tasks (sequence, 16 query heads of a key head) / workgroups, at least min_quota;
+//   if the tasks, cut into pieces of q (or of 9/8 q), are no more pieces than workgroups: one piece each;
+//   else all tasks stand in a row, each with PA_TASK_COST further tiles for what a task costs besides its tiles, and workgroup w takes the
+//   run [w q, (w + 1) q) of the row, whatever the lengths are.
+// A task that lies in one share is finished there; one that is cut leaves a partial sum per workgroup (at most two each: the
+// task that a share begins in the middle of, and the one that it ends in the middle of), and whichever workgroup of a task
+// arrives last joins them in order.
 struct PaSplit {
-    uint32_t* counters;             // [gridDim.x] arrivals of the task that begins in run w and ends behind it; zero between calls
+    uint32_t* counters;             // [gridDim.x] arrivals of the task that begins in share w and ends behind it; zero between calls
     float* partial;                 // [gridDim.x][2][slot], slot: m[16], l[16], o[used][D]
     int slot;
     int min_quota;
     int tasks_a_sequence, head_tiles;
     float c;
 };
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);        // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);        // row_bcast 15: the row in front
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);        // row_bcast 31: the two rows in front
+    return v;
+}
 
 struct PaSequence {
     int lo, hi, first, tiles;       // tokens that count, first tile, number of tiles
@@ -255,54 +359,56 @@ __device__ __forceinline__ PaSequence pa_sequence(const kmi_paged_attn_args& p, 
     return s;
 }
 
-// Sums relative to a maximum, joined over NW waves: wave v adds up the output tiles T = v * OT / NW .. of all of them.
-template <int D, int KIND>
-struct PaJoin {
-    using W = PaWave<D, KIND>;
-    static constexpr int NW = 4, MINE = W::OT / NW;
-    float m[NW][16], l[NW][16];
-    f4_t o[NW][MINE * (NW - 1)][64];            // every wave's tiles but those that it adds up itself
+template <bool V>
+struct Flag {
+    static constexpr bool value = V;
 };
 
-template <int D, int KIND>
-__global__ __launch_bounds__(256) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
-    using W = PaWave<D, KIND>;
-    using J = PaJoin<D, KIND>;
-    constexpr int NW = J::NW, MINE = J::MINE;
+// Sums relative to a maximum, joined over NW waves: wave v adds up the output tiles T = v * OT / NW .. of all of them.
+template <int D, int KIND, int PACK>
+struct PaJoin {
+    using W = PaWave<D, KIND, PACK>;
+    static constexpr int MINE = W::OT / 4;
+    float m[4][16], l[4][16];
+    f4_t o[4][W::OT][64];
+};
+
+template <int D, int KIND, int PACK, int QUARTETS>
+__global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
+    using W = PaWave<D, KIND, PACK>;
+    using J = PaJoin<D, KIND, PACK>;
+    constexpr int NW = 4 * QUARTETS, MINE = J::MINE, DEPTH = PA_DEPTH;
     __shared__ J join;
     __shared__ int last;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int G = p.H / p.KV, run = blockIdx.x;
     half_t* out0 = static_cast<half_t*>(p.out);
 
-    // sequences without a tile: zeros, or NaN where the length does not fit the page table
-    for (int b = run; b < p.B; b += gridDim.x) {
-        const PaSequence s = pa_sequence(p, p.lens[b]);
-        if (s.tiles) continue;
-        const uint32_t fill = s.over ? 0x7E007E00u : 0u;
-        u4_t* o = reinterpret_cast<u4_t*>(out0 + (size_t)b * p.H * D);
-        for (int i = threadIdx.x; i < p.H * D / 8; i += 256) o[i] = u4_t{fill, fill, fill, fill};
+    const int lens0 = lane < p.B ? p.lens[lane] : 0;                       // of the first 64 sequences: most often all
+    auto tiles_of = [&](int b0) {                                          // of sequence b0 + lane
+        const int b = b0 + lane;
+        return b < p.B ? pa_sequence(p, b0 == 0 ? lens0 : p.lens[b]).tiles : 0;
+    };
+    auto sum_over = [&](auto f) {                                          // over the sequences, f(tiles), times the tasks of one
+        int v = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 64) v += __builtin_amdgcn_readlane(wave_scan(f(tiles_of(b0))), 63);
+        return v * sp.tasks_a_sequence;
+    };
+    const int W_ = gridDim.x;
+    auto quota_of = [&](int units) { return (max((units + W_ - 1) / W_, sp.min_quota) + NW - 1) / NW * NW; };
+    int quota = quota_of(sum_over([](int n) { return n; }));
+    auto pieces = [&](int q) { return sum_over([q](int n) { return (n + q - 1) / q; }); };
+    bool even = pieces(quota) <= W_;
+    if (!even) {
+        const int more = (quota + quota / 8 + NW - 1) / NW * NW;
+        even = pieces(more) <= W_;
+        quota = even ? more : quota_of(sum_over([](int n) { return n ? n + PA_TASK_COST : 0; }));
     }
-
-    // all tiles, the run's share, and the sequence that it begins in
-    int total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) total += b0 + lane < p.B ? pa_sequence(p, p.lens[b0 + lane]).tiles : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-    const int U = __builtin_amdgcn_readfirstlane(total) * sp.tasks_a_sequence;
-    int quota = (U + (int)gridDim.x - 1) / (int)gridDim.x;
-    quota = (max(quota, sp.min_quota) + NW - 1) / NW * NW;
-    const int begin = run * quota, end = min(U, begin + quota);
-    if (run > (U - 1) / quota || U == 0) return;
-    int b = 0, before = 0;                                      // before: tiles of the sequences in front, times tasks
+    auto room = [&](int n) { return n == 0 ? 0 : even ? (n + quota - 1) / quota * quota : n + PA_TASK_COST; };     // a task's, in the row
+    const int begin = run * quota, end = begin + quota;
+    int b = p.B, before = 0;                                               // before: the room of the sequences in front
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int mine = b0 + lane < p.B ? pa_sequence(p, p.lens[b0 + lane]).tiles * sp.tasks_a_sequence : 0;
-        int upto = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int v = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += v;
-        }
+        const int mine = room(tiles_of(b0)) * sp.tasks_a_sequence, upto = wave_scan(mine);
         const uint64_t behind = __ballot(before + upto > begin);
         if (behind) {
             const int at = __builtin_ctzll(behind);
@@ -312,22 +418,25 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(kmi_paged_attn_args p, 
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
+    auto len_of = [&](int b) { return b < 64 ? __builtin_amdgcn_readlane(lens0, b & 63) : p.lens[b]; };
 
     for (int unit = begin; unit < end && b < p.B;) {
-        const PaSequence seq = pa_sequence(p, p.lens[b]);
-        if (unit >= before + seq.tiles * sp.tasks_a_sequence) {
-            before += seq.tiles * sp.tasks_a_sequence;
+        const PaSequence seq = pa_sequence(p, len_of(b));
+        const int space = room(seq.tiles);
+        if (unit >= before + space * sp.tasks_a_sequence) {
+            before += space * sp.tasks_a_sequence;
             ++b;
             continue;
         }
-        const int task = (unit - before) / seq.tiles, ta = unit - before - task * seq.tiles;
-        const int tb = min(seq.tiles, ta + end - unit);
-        const int task0 = before + task * seq.tiles;                       // the task's first unit
+        const int task = (unit - before) / space, task0 = before + task * space, ta = unit - task0;
+        const int tb = min(seq.tiles, end - task0);
+        unit = task0 + min(space, end - task0);
+        if (ta >= tb) continue;
         const int head = task / sp.head_tiles, h0 = (task - head * sp.head_tiles) * 16, used = min(16, G - h0);
-        unit += tb - ta;
 
         W w;
-        w.start(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(col, used - 1)) * D, col < used, g);
+        const int hcol = PACK == 2 ? col & 7 : col;                        // the column's query head
+        w.start(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(hcol, used - 1)) * D, hcol < used, col, g, sp.c);
         // this wave's tiles ta + wave + NW i; their places in the pool, 64 at a time, one a lane
         const int count = (tb - ta - wave + NW - 1) / NW;
         const char* cache = static_cast<const char*>(p.cache);
@@ -344,64 +453,95 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(kmi_paged_attn_args p, 
             }
             return __builtin_amdgcn_readlane(places, i & 63);
         };
-        typename W::Tile tile;
-        int place = 0;
-        if (count > 0) {
-            place = place_of(0);
-            const char* at = cache + (size_t)max(place, 0) * W::TILE_BYTES;
-            w.load_keys(tile, at, lane);
-            w.load_values(tile, at, lane);
-        }
-        for (int i = 0; i < count; ++i) {
-            typename W::Scores sc = w.scores(tile);
-            typename W::Factors fac = tile.f;
-            const bool bad = place < 0;
-            const char* next = nullptr;
-            if (i + 1 < count) {
-                place = place_of(i + 1);
-                next = cache + (size_t)max(place, 0) * W::TILE_BYTES;
-                w.load_keys(tile, next, lane);
+        // DEPTH tiles in flight: a tile's registers are loaded again, for DEPTH tiles further on, as soon as they are used up
+        typename W::Tile tile[DEPTH];
+        int place[DEPTH];
+        auto fetch_keys = [&](int s, int i) {
+            place[s] = place_of(i);
+            w.load_keys(tile[s], cache + (size_t)max(place[s], 0) * W::TILE_BYTES, lane);
+        };
+        auto fetch_values = [&](int s) { w.load_values(tile[s], cache + (size_t)max(place[s], 0) * W::TILE_BYTES, lane); };
+#pragma unroll
+        for (int s = 0; s < DEPTH; ++s)
+            if (s < count) {
+                fetch_keys(s, s);
+                fetch_values(s);
             }
+        // (a load under a condition would make the compiler wait for every load wherever it waits for one)
+        auto step = [&](auto more, int s, int i) {
+            typename W::Scores sc = w.scores(tile[s], lane);
+            typename W::Factors fac = tile[s].f;
+            const bool bad = place[s] < 0;
+            if constexpr (more.value) fetch_keys(s, i + DEPTH);
+            PA_SCHED;
             const int t = seq.first + ta + wave + NW * i;
             const bool whole = t * KV_TILE >= seq.lo && (t + 1) * KV_TILE <= seq.hi;
-            const h8_t pf = w.weights(sc, tile.v, fac, t * KV_TILE + 8 * g, seq.lo, seq.hi, whole, bad, sp.c);
-            w.add(tile.v, pf);
-            if (next) w.load_values(tile, next, lane);
+            const h8_t pf = w.weights(sc, tile[s].v, fac, t * KV_TILE, seq.lo, seq.hi, whole, bad, lane);
+            PA_SCHED;                                          // values are decoded where they are used: not before, into registers
+            w.add(tile[s].v, pf);
+            if constexpr (more.value) fetch_values(s);
+            PA_SCHED;
+        };
+        int i = 0;
+        if constexpr (DEPTH == 1) {
+            for (; i + 1 < count; ++i) step(Flag<true>(), 0, i);
+            if (i < count) step(Flag<false>(), 0, i);
+        } else {
+            for (; i + 4 <= count; i += 2) {
+                step(Flag<true>(), 0, i);
+                step(Flag<true>(), 1, i + 1);
+            }
+            if (i + 3 <= count) {
+                step(Flag<true>(), 0, i);
+                step(Flag<false>(), 1, i + 1);
+                step(Flag<false>(), 0, i + 2);
+            } else {
+                if (i < count) step(Flag<false>(), 0, i);
+                if (i + 1 < count) step(Flag<false>(), 1, i + 1);
+            }
         }
 
         // the waves' sums, joined
-        w.l = group_sum(w.l);
-        if constexpr (KIND == KMI_KV_INT4) w.zsum = group_sum(w.zsum);
-        if (g == 0) { join.m[wave][col] = w.m; join.l[wave][col] = w.l; }
-        w.unscale();
-        if (col < used) {
+        w.finish();
 #pragma unroll
-            for (int T = 0; T < W::OT; ++T)
-                if (T / MINE != wave) join.o[wave][T - (T / MINE > wave ? MINE : 0)][lane] = w.acc[T];
+        for (int f = QUARTETS - 1; f >= 0; --f) {              // quartet f hands over to quartet f - 1, the first to itself
+            if (wave / 4 == f) {
+                if (g == 0) { join.m[wave & 3][col] = w.m; join.l[wave & 3][col] = w.l; }
+#pragma unroll
+                for (int T = 0; T < W::OT; ++T) join.o[wave & 3][T][lane] = w.acc[T];
+            }
+            __syncthreads();
+            if (f > 0) {
+                if (wave / 4 == f - 1) {
+                    const float m1 = join.m[wave & 3][col], m2 = fmaxf(w.m, m1);
+                    const float a0 = __builtin_amdgcn_exp2f(w.m - m2), a1 = __builtin_amdgcn_exp2f(m1 - m2);
+                    w.l = w.l * a0 + join.l[wave & 3][col] * a1;
+                    w.m = m2;
+#pragma unroll
+                    for (int T = 0; T < W::OT; ++T) w.acc[T] = w.acc[T] * a0 + join.o[wave & 3][T][lane] * a1;
+                }
+                __syncthreads();
+            }
         }
-        __syncthreads();
-        float mm = PA_NEG, ll = 0.0f, a[NW];
+        float mm = PA_NEG, ll = 0.0f, a[4];
 #pragma unroll
-        for (int v = 0; v < NW; ++v) mm = fmaxf(mm, join.m[v][col]);
+        for (int v = 0; v < 4; ++v) mm = fmaxf(mm, join.m[v][col]);
 #pragma unroll
-        for (int v = 0; v < NW; ++v) {
-            a[v] = __builtin_amdgcn_exp2f((join.m[v][col] - mm) * sp.c);
+        for (int v = 0; v < 4; ++v) {
+            a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
             ll += a[v] * join.l[v][col];
         }
         const bool complete = ta == 0 && tb == seq.tiles;
         float* slot = sp.partial + ((size_t)run * 2 + (ta == 0)) * sp.slot;
         half_t* out = out0 + ((size_t)b * p.H + head * G + h0) * D;
         const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
-        if (col < used) {
+        if (wave < 4 && col < used) {
 #pragma unroll
-            for (int T = 0; T < W::OT; ++T) {
-                if (T / MINE != wave) continue;
+            for (int i = 0; i < MINE; ++i) {
+                const int T = wave * MINE + i;
                 f4_t o = {};
 #pragma unroll
-                for (int v = 0; v < NW; ++v) {
-                    const f4_t x = v == wave ? w.acc[T] : join.o[v][T - (T / MINE > v ? MINE : 0)][lane];
-                    o = o + x * a[v];
-                }
+                for (int v = 0; v < 4; ++v) o = o + join.o[v][T][lane] * a[v];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int d = W::d_of(T, 4 * g + r);
@@ -425,17 +565,20 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(kmi_paged_attn_args p, 
             __syncthreads();
             if (last) {
                 auto slot_of = [&](int v) { return sp.partial + ((size_t)(w0 + v) * 2 + (v == 0)) * sp.slot; };
-                for (int i = threadIdx.x; i < used * D; i += 256) {
+                for (int i = threadIdx.x; i < used * D; i += 64 * NW) {
                     const int hc = i / D;
                     float top = PA_NEG, sum = 0.0f, o = 0.0f;
-#pragma unroll 8
-                    for (int v = 0; v < n; ++v) top = fmaxf(top, __hip_atomic_load(slot_of(v) + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-#pragma unroll 8
+#pragma unroll 4
                     for (int v = 0; v < n; ++v) {
                         const float* s = slot_of(v);
-                        const float f = __builtin_amdgcn_exp2f((__hip_atomic_load(s + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - top) * sp.c);
-                        sum += f * __hip_atomic_load(s + 16 + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        o += f * __hip_atomic_load(s + 32 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        const float mv = __hip_atomic_load(s + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        const float lv = __hip_atomic_load(s + 16 + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        const float ov = __hip_atomic_load(s + 32 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        const float next = fmaxf(top, mv);
+                        const float keep = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(mv - next);
+                        sum = sum * keep + f * lv;
+                        o = o * keep + f * ov;
+                        top = next;
                     }
                     out[i] = (half_t)(sum == 0.0f ? 0.0f : o / sum);
                 }
@@ -443,6 +586,15 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(kmi_paged_attn_args p, 
             }
         }
         __syncthreads();                                       // the next task writes the shared arrays again
+    }
+
+    // sequences without a tile: zeros, or NaN where the length does not fit the page table
+    for (int b = run; b < p.B; b += gridDim.x) {
+        const PaSequence s = pa_sequence(p, len_of(b));
+        if (s.tiles) continue;
+        const uint32_t fill = s.over ? 0x7E007E00u : 0u;
+        u4_t* o = reinterpret_cast<u4_t*>(out0 + (size_t)b * p.H * D);
+        for (int i = threadIdx.x; i < p.H * D / 8; i += 64 * NW) o[i] = u4_t{fill, fill, fill, fill};
     }
 }
 
@@ -471,26 +623,30 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
     sp.min_quota = KMI_PA_MIN_QUOTA;
     sp.counters = static_cast<uint32_t*>(p.workspace);
     sp.partial = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + KMI_GEMV_WS_HEADER);
-    // as many runs as the GPU holds at once, never more than the tasks have room for
+    // as many workgroups as the GPU holds at once, never more than the tasks can be cut into
     const long long most = (long long)p.B * sp.tasks_a_sequence * p.max_pages * p.page_tiles;
     if (most > 0x7FFFFFFFll)
         return kmi_set_error(KMI_E_SHAPE, "%s: %d sequences of %d pages hold more than 2^31 tiles", fn, p.B, p.max_pages);
-    const long long by_quota = (most + sp.min_quota - 1) / sp.min_quota;
-    const int runs = (int)(by_quota < KMI_PA_RUNS ? by_quota : KMI_PA_RUNS);
-    const size_t need = KMI_GEMV_WS_HEADER + (size_t)KMI_PA_RUNS * 2 * sp.slot * sizeof(float);
+    const long long pieces = (long long)p.B * sp.tasks_a_sequence * (((long long)p.max_pages * p.page_tiles + sp.min_quota - 1) / sp.min_quota);
+    const int most_runs = PA_RUNS_EXPR, runs = (int)(pieces < most_runs ? pieces : most_runs);
+    const size_t need = KMI_GEMV_WS_HEADER + (size_t)most_runs * 2 * sp.slot * sizeof(float);
     if (!p.workspace || p.workspace_bytes < need)
         return kmi_set_error(KMI_E_SHAPE, "%s: the workspace must hold %zu bytes (has %zu)", fn, need, p.workspace ? (size_t)p.workspace_bytes : (size_t)0);
-    const dim3 grid(runs), block(256);
+    const int quartets = p.D == 256 ? 1 : PA_QUARTETS;
+    const dim3 grid(runs), block(256 * quartets);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define KMI_PA_LAUNCH(D_)                                                                                             \
-    switch (p.kind) {                                                                                                 \
-        case KMI_KV_F16: hipLaunchKernelGGL((paged_attn_kernel<D_, KMI_KV_F16>), grid, block, 0, st, p, sp); break;   \
-        case KMI_KV_INT8: hipLaunchKernelGGL((paged_attn_kernel<D_, KMI_KV_INT8>), grid, block, 0, st, p, sp); break; \
-        default: hipLaunchKernelGGL((paged_attn_kernel<D_, KMI_KV_INT4>), grid, block, 0, st, p, sp);                 \
+#define KMI_PA_KIND(D_, K_) \
+    hipLaunchKernelGGL((G <= 8 && K_ != KMI_KV_F16 ? paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, D_ == 256 ? 1 : PA_QUARTETS> : paged_attn_kernel<D_, K_, 1, D_ == 256 ? 1 : PA_QUARTETS>), grid, block, PA_LDS, st, p, sp)
+#define KMI_PA_LAUNCH(D_)                                          \
+    switch (p.kind) {                                              \
+        case KMI_KV_F16: KMI_PA_KIND(D_, KMI_KV_F16); break;       \
+        case KMI_KV_INT8: KMI_PA_KIND(D_, KMI_KV_INT8); break;     \
+        default: KMI_PA_KIND(D_, KMI_KV_INT4);                     \
     }
     if (p.D == 64) { KMI_PA_LAUNCH(64) }
     else if (p.D == 128) { KMI_PA_LAUNCH(128) }
     else { KMI_PA_LAUNCH(256) }
 #undef KMI_PA_LAUNCH
+#undef KMI_PA_KIND
     return kmi_check_launch(fn);
 }
