@@ -12,38 +12,20 @@
 // more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to one scalar a head.
 #include "kv_parts.h"
 
-#ifndef PA_RUNS_EXPR
-#define PA_RUNS_EXPR 256
+#ifndef PA_MIN_STEPS
+#define PA_MIN_STEPS 4
 #endif
-#ifndef PA_QUARTETS
-#define PA_QUARTETS 2
+#ifndef PA_NW
+#define PA_NW 4
 #endif
-#ifndef PA_BOUND
-#define PA_BOUND 1
-#endif
-#ifndef PA_DEPTH
-#define PA_DEPTH 1
-#endif
-#ifndef PA_SCHED
-#define PA_SCHED __builtin_amdgcn_sched_barrier(0)
-#endif
-#ifndef PA_LDS
-#define PA_LDS 0
-#endif
-#ifndef PA_R64
-#define PA_R64 4
-#endif
-#ifndef PA_R128
-#define PA_R128 3
-#endif
-// Workgroups (four waves) that a CU holds at once: what the registers of the accumulators, the operand of q and a tile in flight leave.
-static constexpr int pa_resident(int D) { return D == 64 ? PA_R64 : D == 128 ? PA_R128 : 2; }
-#ifndef KMI_PA_MIN_QUOTA
-#define KMI_PA_MIN_QUOTA 8
-#endif
-
 #ifndef PA_TASK_COST
 #define PA_TASK_COST 6
+#endif
+#ifndef PA_LONG
+#define PA_LONG 96
+#endif
+#ifndef PA_U
+#define PA_U (kv_tile_bytes(D, KIND) < 8500 && D < 256 ? 2 : 1)
 #endif
 
 static constexpr float PA_NEG = -1e30f;       // running maximum before the first token: finite, so differences stay numbers
@@ -103,6 +85,7 @@ struct PaWave {
     static constexpr int n = kv_per_word(KIND), CH = D / 16 / n, KSTEPS = D / 32, OT = D / 16, NF = kv_factors(KIND);
     static constexpr int TILE_BYTES = kv_tile_bytes(D, KIND), PART = kv_part_bytes(D, KIND);
     static constexpr int NS = 8 / PACK;                        // scores a lane holds of a tile
+    static constexpr int U = PA_U;                             // tiles a step: independent chains of products and exponentials
     static constexpr bool CODES = KIND != KMI_KV_F16;
     typedef _Float16 fac_t __attribute__((ext_vector_type(NS)));
     h8_t q[PACK][KSTEPS];       // lane (column, g): q[32 kk + 8 g ..]
@@ -112,11 +95,15 @@ struct PaWave {
     float l, zsum;              // this lane's share of the sums of p and of p * offset
     float c, qc;                // scale * log2(e), for codes times 2^24 (their unit); sum of q, times scale * log2(e)
 
-    __device__ __forceinline__ void start(const half_t* qrow, bool used, int col, int g, float scale) {
+    __device__ __forceinline__ void load_q(const half_t* qrow, bool used, int g) {
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) q[0][kk] = used ? *reinterpret_cast<const h8_t*>(qrow + 32 * kk + 8 * g) : h8_t{};
+    }
+    __device__ __forceinline__ void start(int col, float scale) {
         float s = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) {
-            h8_t x = used ? *reinterpret_cast<const h8_t*>(qrow + 32 * kk + 8 * g) : h8_t{};
+            h8_t x = q[0][kk];
             if constexpr (CODES) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s += (float)x[e];
@@ -149,6 +136,9 @@ struct PaWave {
     };
     struct Scores {
         float s[NS];
+    };
+    struct Operand {
+        h8_t p[U];
     };
     // The first of the lane's NS tokens in a tile.
     static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
@@ -193,58 +183,68 @@ struct PaWave {
     // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
     // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (to the largest x plus
     // the logarithm of the largest value scale) only where a weight would pass 2^10 or p 2^40, which is seldom after a wave's
-    // first tile: no reduction over lanes otherwise.  val: the tile's values, fac: its factors, tok: its first token, [lo, hi)
-    // the tokens that count, whole: the tile lies inside, bad: no page of this cache.
-    __device__ __forceinline__ h8_t weights(const Scores& sc, u4_t (&val)[CH], Factors& fac, int tok, int lo, int hi, bool whole, bool bad,
-                                            int lane) {
-        float vs[NS], y[NS], p[NS], wt[NS];
+    // first tile: no reduction over lanes otherwise.  fac: the tiles' factors, tok: the first tile's first token, [lo, hi) the
+    // tokens that count, bad: no page of this cache.
+    __device__ __forceinline__ Operand weights(const Scores (&sc)[U], Tile (&tile)[U], Factors (&fac)[U], int tok, int lo, int hi,
+                                               const bool (&bad)[U], int lane) {
+        float vs[U][NS], y[U][NS], p[U][NS], wt[U][NS];
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            vs[j] = CODES ? (float)fac.f[NF / 2][j] : 1.0f;
-            y[j] = exponent(sc.s[j], fac, j, m);
-        }
-        if (!whole) {
-            // tokens outside: no weight, and nothing that stands in their place may reach a product
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                const int t = tok + first_token(lane) + j;
-                const bool in = t >= lo && t < hi;
-                y[j] = in ? y[j] : -__builtin_inff();
-                vs[j] = in ? vs[j] : 0.0f;
-                if constexpr (KIND == KMI_KV_INT4) fac.f[3][j] = in ? fac.f[3][j] : (half_t)0.0f;
+                vs[u][j] = CODES ? (float)fac[u].f[NF / 2][j] : 1.0f;
+                y[u][j] = exponent(sc[u].s[j], fac[u], j, m);
             }
-            if constexpr (!CODES) {
-                u4_t keep = {};
+        if (tok < lo || tok + U * KV_TILE > hi) {
+            // tokens outside: no weight, and nothing that stands in their place may reach a product
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int t = tok + 8 * (lane >> 4) + j;
-                    keep[j >> 1] |= t >= lo && t < hi ? 0xFFFFu << (16 * (j & 1)) : 0u;
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const int t = tok + u * KV_TILE + first_token(lane) + j;
+                    const bool in = t >= lo && t < hi;
+                    y[u][j] = in ? y[u][j] : -__builtin_inff();
+                    vs[u][j] = in ? vs[u][j] : 0.0f;
+                    if constexpr (KIND == KMI_KV_INT4) fac[u].f[3][j] = in ? fac[u].f[3][j] : (half_t)0.0f;
                 }
+                if constexpr (!CODES) {
+                    u4_t keep = {};
 #pragma unroll
-                for (int i = 0; i < CH; ++i) val[i] &= keep;
+                    for (int j = 0; j < 8; ++j) {
+                        const int t = tok + u * KV_TILE + 8 * (lane >> 4) + j;
+                        keep[j >> 1] |= t >= lo && t < hi ? 0xFFFFu << (16 * (j & 1)) : 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) tile[u].v[i] &= keep;
+                }
             }
-        }
-        if (bad) {
-#pragma unroll
-            for (int j = 0; j < NS; ++j) y[j] = __builtin_nanf("");
         }
         float wtop = 0.0f, ytop = PA_NEG;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(y[j]);
-            wt[j] = CODES ? p[j] * vs[j] : p[j];
-            wtop = fmaxf(wtop, wt[j]);
-            if constexpr (CODES) ytop = fmaxf(ytop, y[j]);
+        for (int u = 0; u < U; ++u) {
+            if (bad[u]) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j) y[u][j] = __builtin_nanf("");
+            }
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                p[u][j] = __builtin_amdgcn_exp2f(y[u][j]);
+                wt[u][j] = CODES ? p[u][j] * vs[u][j] : p[u][j];
+                wtop = fmaxf(wtop, wt[u][j]);
+                if constexpr (CODES) ytop = fmaxf(ytop, y[u][j]);
+            }
         }
         if (__any(wtop > 1024.0f || ytop > 40.0f)) {
             float top = -__builtin_inff(), vtop = 0x1p-24f;
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                // from the products again: y is what m left of x
-                y[j] = y[j] == -__builtin_inff() ? y[j] : exponent(sc.s[j], fac, j, 0.0f);
-                top = fmaxf(top, y[j]);
-                vtop = fmaxf(vtop, vs[j]);
-            }
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    // from the products again: y is what m left of x
+                    y[u][j] = y[u][j] == -__builtin_inff() ? y[u][j] : bad[u] ? __builtin_nanf("") : exponent(sc[u].s[j], fac[u], j, 0.0f);
+                    top = fmaxf(top, y[u][j]);
+                    vtop = fmaxf(vtop, vs[u][j]);
+                }
             top = group_max(top);
             if constexpr (CODES) top += __builtin_amdgcn_logf(group_max(vtop));
             const float m2 = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - m2);
@@ -254,32 +254,42 @@ struct PaWave {
 #pragma unroll
             for (int i = 0; i < OT; ++i) acc[i] = acc[i] * a;
 #pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    p[u][j] = __builtin_amdgcn_exp2f(y[u][j] - m);
+                    wt[u][j] = CODES ? p[u][j] * vs[u][j] : p[u][j];
+                }
+        }
+        Operand o;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            h8_t pf = {};
+#pragma unroll
             for (int j = 0; j < NS; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(y[j] - m);
-                wt[j] = CODES ? p[j] * vs[j] : p[j];
+                l += p[u][j];
+                if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[u][j], __builtin_fmaf(8.0f, vs[u][j], (float)fac[u].f[3][j]), zsum);
+                pf[j] = (half_t)wt[u][j];
             }
+            if constexpr (PACK == 2) {                         // the lane's tokens are its column's half of the operand's eight
+                const u4_t w = __builtin_bit_cast(u4_t, pf);
+                const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
+                pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
+            }
+            o.p[u] = pf;
         }
-        h8_t pf = {};
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            l += p[j];
-            if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(8.0f, vs[j], (float)fac.f[3][j]), zsum);
-            pf[j] = (half_t)wt[j];
-        }
-        if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
-            const u4_t w = __builtin_bit_cast(u4_t, pf);
-            const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
-            pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
-        }
-        return pf;
+        return o;
     }
-    __device__ __forceinline__ void add(const u4_t (&val)[CH], const h8_t& pf) {
+    __device__ __forceinline__ void add(const Tile (&tile)[U], const Operand& w) {
 #pragma unroll
-        for (int T = 0; T < OT; ++T)
-            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(val[T / n], T % n), pf, acc[T], 0, 0, 0);
-        if constexpr (CODES) {
-            const half_t one = (half_t)1.0f;
-            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, pf, psum, 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int T = 0; T < OT; ++T)
+                acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(tile[u].v[T / n], T % n), w.p[u], acc[T], 0, 0, 0);
+            if constexpr (CODES) {
+                const half_t one = (half_t)1.0f;
+                psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w.p[u], psum, 0, 0, 0);
+            }
         }
     }
     // The sums as they stand: over the lane groups, and for codes the units, the codes' middle (taken off with the very
@@ -328,7 +338,6 @@ struct PaSplit {
     uint32_t* counters;             // [gridDim.x] arrivals of the task that begins in share w and ends behind it; zero between calls
     float* partial;                 // [gridDim.x][2][slot], slot: m[16], l[16], o[used][D]
     int slot;
-    int min_quota;
     int tasks_a_sequence, head_tiles;
     float c;
 };
@@ -373,11 +382,11 @@ struct PaJoin {
     f4_t o[4][W::OT][64];
 };
 
-template <int D, int KIND, int PACK, int QUARTETS>
-__global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
+template <int D, int KIND, int PACK, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
     using W = PaWave<D, KIND, PACK>;
     using J = PaJoin<D, KIND, PACK>;
-    constexpr int NW = 4 * QUARTETS, MINE = J::MINE, DEPTH = PA_DEPTH;
+    constexpr int MINE = J::MINE, U = W::U;
     __shared__ J join;
     __shared__ int last;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
@@ -394,18 +403,31 @@ __global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(km
         for (int b0 = 0; b0 < p.B; b0 += 64) v += __builtin_amdgcn_readlane(wave_scan(f(tiles_of(b0))), 63);
         return v * sp.tasks_a_sequence;
     };
-    const int W_ = gridDim.x;
-    auto quota_of = [&](int units) { return (max((units + W_ - 1) / W_, sp.min_quota) + NW - 1) / NW * NW; };
-    int quota = quota_of(sum_over([](int n) { return n; }));
-    auto pieces = [&](int q) { return sum_over([q](int n) { return (n + q - 1) / q; }); };
-    bool even = pieces(quota) <= W_;
-    if (!even) {
-        const int more = (quota + quota / 8 + NW - 1) / NW * NW;
-        even = pieces(more) <= W_;
-        quota = even ? more : quota_of(sum_over([](int n) { return n ? n + PA_TASK_COST : 0; }));
+    // One workgroup a CU where the shares come out even or are long, else as many as there are.
+    constexpr int STEP = NW * U;                                           // tiles a workgroup takes at once
+    const int units = sum_over([](int n) { return n; }), most = gridDim.x;
+    auto quota_of = [&](int units, int shares) { return (max((units + shares - 1) / shares, PA_MIN_STEPS * STEP) + STEP - 1) / STEP * STEP; };
+    auto pieces_of = [](int n, int q) { return n <= PA_MIN_STEPS * STEP * 3 / 2 ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
+    auto pieces = [&](int q) { return sum_over([&](int n) { return pieces_of(n, q); }); };
+    int shares = min(most, 256), quota = quota_of(units, shares);
+    bool even = pieces(quota) <= shares;
+    for (int pass = 0; !even; ++pass) {
+        const int more = (quota + quota / 8 + STEP - 1) / STEP * STEP;
+        even = pieces(more) <= shares;
+        if (even) {
+            quota = more;
+        } else if (pass == 1 || quota >= PA_LONG || shares == most) {
+            quota = quota_of(sum_over([](int n) { return n ? n + PA_TASK_COST : 0; }), shares);
+            break;
+        } else {
+            shares = most;
+            quota = quota_of(units, shares);
+            even = pieces(quota) <= shares;
+        }
     }
-    auto room = [&](int n) { return n == 0 ? 0 : even ? (n + quota - 1) / quota * quota : n + PA_TASK_COST; };     // a task's, in the row
-    const int begin = run * quota, end = begin + quota;
+    // the row that the shares are cut from: pieces, one a share, or tiles and PA_TASK_COST a task, `quota` a share
+    auto room = [&](int n) { return n == 0 ? 0 : even ? pieces_of(n, quota) : n + PA_TASK_COST; };     // a task's, in the row
+    const int per_share = even ? 1 : quota, begin = run * per_share, end = begin + per_share;
     int b = p.B, before = 0;                                               // before: the room of the sequences in front
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int mine = room(tiles_of(b0)) * sp.tasks_a_sequence, upto = wave_scan(mine);
@@ -428,83 +450,90 @@ __global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(km
             ++b;
             continue;
         }
-        const int task = (unit - before) / space, task0 = before + task * space, ta = unit - task0;
-        const int tb = min(seq.tiles, end - task0);
-        unit = task0 + min(space, end - task0);
-        if (ta >= tb) continue;
+        const int task = (unit - before) / space, task0 = before + task * space;
+        int ta = unit - task0, tb, first_share = run, parts = 1;           // the share's tiles of the task; the task's shares
+        if (even) {
+            first_share = task0;
+            parts = space;
+            tb = (int)((long)(ta + 1) * seq.tiles / space);
+            ta = (int)((long)ta * seq.tiles / space);
+            unit = end;
+        } else {
+            tb = min(seq.tiles, end - task0);
+            unit = task0 + min(space, end - task0);
+            if (ta >= tb) continue;
+            first_share = task0 / quota;
+            parts = (task0 + seq.tiles - 1) / quota - first_share + 1;
+        }
         const int head = task / sp.head_tiles, h0 = (task - head * sp.head_tiles) * 16, used = min(16, G - h0);
 
         W w;
         const int hcol = PACK == 2 ? col & 7 : col;                        // the column's query head
-        w.start(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(hcol, used - 1)) * D, hcol < used, col, g, sp.c);
-        // this wave's tiles ta + wave + NW i; their places in the pool, 64 at a time, one a lane
-        const int count = (tb - ta - wave + NW - 1) / NW;
+        w.load_q(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(hcol, used - 1)) * D, hcol < used, g);
+        // this wave's steps: U neighbouring tiles each, from ta + U (wave + NW i); behind tb the last tile again, masked.  The
+        // tiles' places in the pool: 64 at a time, one a lane
+        const int count = (tb - ta - wave * U + NW * U - 1) / (NW * U);
+        const int hi = min(seq.hi, (seq.first + tb) * KV_TILE);
         const char* cache = static_cast<const char*>(p.cache);
         int places = -1;
-        auto place_of = [&](int i) {
-            if ((i & 63) == 0) {
-                const int t = seq.first + ta + wave + NW * (i + lane);
+        auto place_of = [&](int k) {                                       // of tile k of the wave
+            if ((k & 63) == 0) {
+                const int t = seq.first + min(ta + ((k + lane) / U * NW + wave) * U + (k + lane) % U, tb - 1);
+                const int page = t / p.page_tiles;
                 places = -1;
-                if (i + lane < count) {
-                    const int page = t / p.page_tiles;
+                if (page < p.max_pages) {
                     const int id = p.page_table[(size_t)b * p.max_pages + page];
                     if (id >= 0 && id < p.num_pages) places = (id * p.KV + head) * p.page_tiles + t - page * p.page_tiles;
                 }
             }
-            return __builtin_amdgcn_readlane(places, i & 63);
+            return __builtin_amdgcn_readlane(places, k & 63);
         };
-        // DEPTH tiles in flight: a tile's registers are loaded again, for DEPTH tiles further on, as soon as they are used up
-        typename W::Tile tile[DEPTH];
-        int place[DEPTH];
-        auto fetch_keys = [&](int s, int i) {
-            place[s] = place_of(i);
-            w.load_keys(tile[s], cache + (size_t)max(place[s], 0) * W::TILE_BYTES, lane);
-        };
-        auto fetch_values = [&](int s) { w.load_values(tile[s], cache + (size_t)max(place[s], 0) * W::TILE_BYTES, lane); };
+        // the registers of a step's keys, then of its values, are loaded for the next step as soon as they are used up
+        typename W::Tile tile[U];
+        int place[U];
+        auto fetch_keys = [&](int i) {
 #pragma unroll
-        for (int s = 0; s < DEPTH; ++s)
-            if (s < count) {
-                fetch_keys(s, s);
-                fetch_values(s);
+            for (int u = 0; u < U; ++u) {
+                place[u] = place_of(i * U + u);
+                w.load_keys(tile[u], cache + (size_t)max(place[u], 0) * W::TILE_BYTES, lane);
             }
+        };
+        auto fetch_values = [&]() {
+#pragma unroll
+            for (int u = 0; u < U; ++u) w.load_values(tile[u], cache + (size_t)max(place[u], 0) * W::TILE_BYTES, lane);
+        };
+        if (count > 0) {
+            fetch_keys(0);
+            fetch_values();
+        }
+        w.start(col, sp.c);
         // (a load under a condition would make the compiler wait for every load wherever it waits for one)
-        auto step = [&](auto more, int s, int i) {
-            typename W::Scores sc = w.scores(tile[s], lane);
-            typename W::Factors fac = tile[s].f;
-            const bool bad = place[s] < 0;
-            if constexpr (more.value) fetch_keys(s, i + DEPTH);
-            PA_SCHED;
-            const int t = seq.first + ta + wave + NW * i;
-            const bool whole = t * KV_TILE >= seq.lo && (t + 1) * KV_TILE <= seq.hi;
-            const h8_t pf = w.weights(sc, tile[s].v, fac, t * KV_TILE, seq.lo, seq.hi, whole, bad, lane);
-            PA_SCHED;                                          // values are decoded where they are used: not before, into registers
-            w.add(tile[s].v, pf);
-            if constexpr (more.value) fetch_values(s);
-            PA_SCHED;
+        auto step = [&](auto more, int i) {
+            typename W::Scores sc[U];
+            typename W::Factors fac[U];
+            bool bad[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                sc[u] = w.scores(tile[u], lane);
+                fac[u] = tile[u].f;
+                bad[u] = place[u] < 0;
+            }
+            if constexpr (more.value) fetch_keys(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const typename W::Operand o = w.weights(sc, tile, fac, (seq.first + ta + (wave + NW * i) * U) * KV_TILE, seq.lo, hi, bad, lane);
+            __builtin_amdgcn_sched_barrier(0);                 // values are decoded where they are used: not before, into registers
+            w.add(tile, o);
+            if constexpr (more.value) fetch_values();
+            __builtin_amdgcn_sched_barrier(0);
         };
         int i = 0;
-        if constexpr (DEPTH == 1) {
-            for (; i + 1 < count; ++i) step(Flag<true>(), 0, i);
-            if (i < count) step(Flag<false>(), 0, i);
-        } else {
-            for (; i + 4 <= count; i += 2) {
-                step(Flag<true>(), 0, i);
-                step(Flag<true>(), 1, i + 1);
-            }
-            if (i + 3 <= count) {
-                step(Flag<true>(), 0, i);
-                step(Flag<false>(), 1, i + 1);
-                step(Flag<false>(), 0, i + 2);
-            } else {
-                if (i < count) step(Flag<false>(), 0, i);
-                if (i + 1 < count) step(Flag<false>(), 1, i + 1);
-            }
-        }
+        for (; i + 1 < count; ++i) step(Flag<true>(), i);
+        if (i < count) step(Flag<false>(), i);
 
         // the waves' sums, joined
         w.finish();
 #pragma unroll
-        for (int f = QUARTETS - 1; f >= 0; --f) {              // quartet f hands over to quartet f - 1, the first to itself
+        for (int f = NW / 4 - 1; f >= 0; --f) {                // four waves at a time: the second four hand over to the first
             if (wave / 4 == f) {
                 if (g == 0) { join.m[wave & 3][col] = w.m; join.l[wave & 3][col] = w.l; }
 #pragma unroll
@@ -531,7 +560,7 @@ __global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(km
             a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
             ll += a[v] * join.l[v][col];
         }
-        const bool complete = ta == 0 && tb == seq.tiles;
+        const bool complete = parts == 1;
         float* slot = sp.partial + ((size_t)run * 2 + (ta == 0)) * sp.slot;
         half_t* out = out0 + ((size_t)b * p.H + head * G + h0) * D;
         const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -558,7 +587,7 @@ __global__ __launch_bounds__(256 * QUARTETS, PA_BOUND) void paged_attn_kernel(km
         if (!complete) {
             // Hand-off without fences: partial sums travel by agent-scope stores and loads, performed at the memory side; every
             // thread waits for its own to be performed, the barrier for every thread, and only then the arrival is counted there.
-            const int w0 = task0 / quota, n = (task0 + seq.tiles - 1) / quota - w0 + 1;
+            const int w0 = first_share, n = parts;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (threadIdx.x == 0) last = __hip_atomic_fetch_add(sp.counters + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(n - 1);
@@ -620,23 +649,21 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
     sp.tasks_a_sequence = p.KV * sp.head_tiles;
     sp.c = p.scale * 1.44269504088896340736f;
     sp.slot = 32 + used * p.D;
-    sp.min_quota = KMI_PA_MIN_QUOTA;
     sp.counters = static_cast<uint32_t*>(p.workspace);
     sp.partial = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + KMI_GEMV_WS_HEADER);
     // as many workgroups as the GPU holds at once, never more than the tasks can be cut into
     const long long most = (long long)p.B * sp.tasks_a_sequence * p.max_pages * p.page_tiles;
     if (most > 0x7FFFFFFFll)
         return kmi_set_error(KMI_E_SHAPE, "%s: %d sequences of %d pages hold more than 2^31 tiles", fn, p.B, p.max_pages);
-    const long long pieces = (long long)p.B * sp.tasks_a_sequence * (((long long)p.max_pages * p.page_tiles + sp.min_quota - 1) / sp.min_quota);
-    const int most_runs = PA_RUNS_EXPR, runs = (int)(pieces < most_runs ? pieces : most_runs);
+    const long long pieces = (long long)p.B * sp.tasks_a_sequence * (((long long)p.max_pages * p.page_tiles + 7) / 8);
+    const int most_runs = PA_NW == 8 ? 256 : 512, runs = (int)(pieces < most_runs ? pieces : most_runs);
     const size_t need = KMI_GEMV_WS_HEADER + (size_t)most_runs * 2 * sp.slot * sizeof(float);
     if (!p.workspace || p.workspace_bytes < need)
         return kmi_set_error(KMI_E_SHAPE, "%s: the workspace must hold %zu bytes (has %zu)", fn, need, p.workspace ? (size_t)p.workspace_bytes : (size_t)0);
-    const int quartets = p.D == 256 ? 1 : PA_QUARTETS;
-    const dim3 grid(runs), block(256 * quartets);
+    const dim3 grid(runs), block(PA_NW * 64);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define KMI_PA_KIND(D_, K_) \
-    hipLaunchKernelGGL((G <= 8 && K_ != KMI_KV_F16 ? paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, D_ == 256 ? 1 : PA_QUARTETS> : paged_attn_kernel<D_, K_, 1, D_ == 256 ? 1 : PA_QUARTETS>), grid, block, PA_LDS, st, p, sp)
+    hipLaunchKernelGGL((G <= 8 && K_ != KMI_KV_F16 ? paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, PA_NW> : paged_attn_kernel<D_, K_, 1, PA_NW>), grid, block, 0, st, p, sp)
 #define KMI_PA_LAUNCH(D_)                                          \
     switch (p.kind) {                                              \
         case KMI_KV_F16: KMI_PA_KIND(D_, KMI_KV_F16); break;       \
