@@ -12,21 +12,19 @@
 // more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to one scalar a head.
 #include "kv_parts.h"
 
-#ifndef PA_MIN_STEPS
-#define PA_MIN_STEPS 4
-#endif
-#ifndef PA_NW
-#define PA_NW 4
-#endif
-#ifndef PA_TASK_COST
-#define PA_TASK_COST 6
-#endif
-#ifndef PA_LONG
-#define PA_LONG 96
-#endif
-#ifndef PA_U
-#define PA_U (kv_tile_bytes(D, KIND) < 8500 && D < 256 ? 2 : 1)
-#endif
+// Waves of a workgroup, one workgroup a CU.  int4 tiles are small and cost as much vector work as the others: eight waves
+// (two a SIMD, one computing while the other waits) read 4 x 100001 tokens in 84 us, four in 97; for int8 and f16 four read as fast (182
+// and 184 us for 2 x 131072 f16) and start and end a share sooner (32 x 1536 int8: 19.8 us against 20.3).
+static constexpr int pa_waves(int kind) { return kind == KMI_KV_INT4 ? 8 : 4; }
+// Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (182 us against 191 for 2 x 131072 f16: fewer places of
+// memory at once), 512 hide the starts and ends of short tasks (19 sequences of up to 7985, int8, 64 wide: 20 us against 29).
+static constexpr int PA_LONG = 96;            // tiles a share from which 256 uneven ones are taken all the same
+// A share below six tiles a wave does not pay its join, which costs about 5 us (511 tokens of 8 heads, int4: 9.0 us whole, 11.4 cut).
+static constexpr int PA_MIN_STEPS = 6;
+static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start and end; 3 and 12 measured the same
+// Tiles of the page table from which a wave takes 32 query heads at once (more than 16 share a key head): the cache is read once
+// (64 x 62479 int8, 20 heads: 115 us against 176), but there are half as many shares (13 x up to 7411 int4: 21 us against 14).
+static constexpr long long PA_WIDE = 12288;
 
 static constexpr float PA_NEG = -1e30f;       // running maximum before the first token: finite, so differences stay numbers
 
@@ -85,7 +83,6 @@ struct PaWave {
     static constexpr int n = kv_per_word(KIND), CH = D / 16 / n, KSTEPS = D / 32, OT = D / 16, NF = kv_factors(KIND);
     static constexpr int TILE_BYTES = kv_tile_bytes(D, KIND), PART = kv_part_bytes(D, KIND);
     static constexpr int NS = 8 / PACK;                        // scores a lane holds of a tile
-    static constexpr int U = PA_U;                             // tiles a step: independent chains of products and exponentials
     static constexpr bool CODES = KIND != KMI_KV_F16;
     typedef _Float16 fac_t __attribute__((ext_vector_type(NS)));
     h8_t q[PACK][KSTEPS];       // lane (column, g): q[32 kk + 8 g ..]
@@ -137,19 +134,16 @@ struct PaWave {
     struct Scores {
         float s[NS];
     };
-    struct Operand {
-        h8_t p[U];
-    };
     // The first of the lane's NS tokens in a tile.
     static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
 
-    __device__ __forceinline__ void load_keys(Tile& t, const char* tile, int lane) const {
+    static __device__ __forceinline__ void load_keys(Tile& t, const char* tile, int lane) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) t.k[i] = *reinterpret_cast<const u4_t*>(tile + i * 1024 + lane * 16);
 #pragma unroll
         for (int i = 0; i < NF; ++i) t.f.f[i] = *reinterpret_cast<const fac_t*>(tile + 2 * PART + 64 * i + 2 * first_token(lane));
     }
-    __device__ __forceinline__ void load_values(Tile& t, const char* tile, int lane) const {
+    static __device__ __forceinline__ void load_values(Tile& t, const char* tile, int lane) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) t.v[i] = *reinterpret_cast<const u4_t*>(tile + PART + i * 1024 + lane * 16);
     }
@@ -183,68 +177,57 @@ struct PaWave {
     // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
     // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (to the largest x plus
     // the logarithm of the largest value scale) only where a weight would pass 2^10 or p 2^40, which is seldom after a wave's
-    // first tile: no reduction over lanes otherwise.  fac: the tiles' factors, tok: the first tile's first token, [lo, hi) the
+    // first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
     // tokens that count, bad: no page of this cache.
-    __device__ __forceinline__ Operand weights(const Scores (&sc)[U], Tile (&tile)[U], Factors (&fac)[U], int tok, int lo, int hi,
-                                               const bool (&bad)[U], int lane) {
-        float vs[U][NS], y[U][NS], p[U][NS], wt[U][NS];
+    __device__ __forceinline__ h8_t weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
+        float vs[NS], y[NS], p[NS], wt[NS];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                vs[u][j] = CODES ? (float)fac[u].f[NF / 2][j] : 1.0f;
-                y[u][j] = exponent(sc[u].s[j], fac[u], j, m);
-            }
-        if (tok < lo || tok + U * KV_TILE > hi) {
+        for (int j = 0; j < NS; ++j) {
+            vs[j] = CODES ? (float)fac.f[NF / 2][j] : 1.0f;
+            y[j] = exponent(sc.s[j], fac, j, m);
+        }
+        if (tok < lo || tok + KV_TILE > hi) {
             // tokens outside: no weight, and nothing that stands in their place may reach a product
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    const int t = tok + u * KV_TILE + first_token(lane) + j;
-                    const bool in = t >= lo && t < hi;
-                    y[u][j] = in ? y[u][j] : -__builtin_inff();
-                    vs[u][j] = in ? vs[u][j] : 0.0f;
-                    if constexpr (KIND == KMI_KV_INT4) fac[u].f[3][j] = in ? fac[u].f[3][j] : (half_t)0.0f;
-                }
-                if constexpr (!CODES) {
-                    u4_t keep = {};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int t = tok + u * KV_TILE + 8 * (lane >> 4) + j;
-                        keep[j >> 1] |= t >= lo && t < hi ? 0xFFFFu << (16 * (j & 1)) : 0u;
-                    }
-#pragma unroll
-                    for (int i = 0; i < CH; ++i) tile[u].v[i] &= keep;
-                }
+            for (int j = 0; j < NS; ++j) {
+                const int t = tok + first_token(lane) + j;
+                const bool in = t >= lo && t < hi;
+                y[j] = in ? y[j] : -__builtin_inff();
+                vs[j] = in ? vs[j] : 0.0f;
+                if constexpr (KIND == KMI_KV_INT4) fac.f[3][j] = in ? fac.f[3][j] : (half_t)0.0f;
             }
+            if constexpr (!CODES) {
+                u4_t keep = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int t = tok + 8 * (lane >> 4) + j;
+                    keep[j >> 1] |= t >= lo && t < hi ? 0xFFFFu << (16 * (j & 1)) : 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < CH; ++i) tile.v[i] &= keep;
+            }
+        }
+        if (bad) {
+#pragma unroll
+            for (int j = 0; j < NS; ++j) y[j] = __builtin_nanf("");
         }
         float wtop = 0.0f, ytop = PA_NEG;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (bad[u]) {
-#pragma unroll
-                for (int j = 0; j < NS; ++j) y[u][j] = __builtin_nanf("");
-            }
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                p[u][j] = __builtin_amdgcn_exp2f(y[u][j]);
-                wt[u][j] = CODES ? p[u][j] * vs[u][j] : p[u][j];
-                wtop = fmaxf(wtop, wt[u][j]);
-                if constexpr (CODES) ytop = fmaxf(ytop, y[u][j]);
-            }
+        for (int j = 0; j < NS; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(y[j]);
+            wt[j] = CODES ? p[j] * vs[j] : p[j];
+            wtop = fmaxf(wtop, wt[j]);
+            if constexpr (CODES) ytop = fmaxf(ytop, y[j]);
         }
         if (__any(wtop > 1024.0f || ytop > 40.0f)) {
             float top = -__builtin_inff(), vtop = 0x1p-24f;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    // from the products again: y is what m left of x
-                    y[u][j] = y[u][j] == -__builtin_inff() ? y[u][j] : bad[u] ? __builtin_nanf("") : exponent(sc[u].s[j], fac[u], j, 0.0f);
-                    top = fmaxf(top, y[u][j]);
-                    vtop = fmaxf(vtop, vs[u][j]);
-                }
+            for (int j = 0; j < NS; ++j) {
+                // from the products again: y is what m left of x
+                y[j] = y[j] == -__builtin_inff() ? y[j] : bad ? __builtin_nanf("") : exponent(sc.s[j], fac, j, 0.0f);
+                top = fmaxf(top, y[j]);
+                vtop = fmaxf(vtop, vs[j]);
+            }
             top = group_max(top);
             if constexpr (CODES) top += __builtin_amdgcn_logf(group_max(vtop));
             const float m2 = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - m2);
@@ -254,42 +237,32 @@ struct PaWave {
 #pragma unroll
             for (int i = 0; i < OT; ++i) acc[i] = acc[i] * a;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    p[u][j] = __builtin_amdgcn_exp2f(y[u][j] - m);
-                    wt[u][j] = CODES ? p[u][j] * vs[u][j] : p[u][j];
-                }
-        }
-        Operand o;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            h8_t pf = {};
-#pragma unroll
             for (int j = 0; j < NS; ++j) {
-                l += p[u][j];
-                if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[u][j], __builtin_fmaf(8.0f, vs[u][j], (float)fac[u].f[3][j]), zsum);
-                pf[j] = (half_t)wt[u][j];
+                p[j] = __builtin_amdgcn_exp2f(y[j] - m);
+                wt[j] = CODES ? p[j] * vs[j] : p[j];
             }
-            if constexpr (PACK == 2) {                         // the lane's tokens are its column's half of the operand's eight
-                const u4_t w = __builtin_bit_cast(u4_t, pf);
-                const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
-                pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
-            }
-            o.p[u] = pf;
         }
-        return o;
+        h8_t pf = {};
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            l += p[j];
+            if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(8.0f, vs[j], (float)fac.f[3][j]), zsum);
+            pf[j] = (half_t)wt[j];
+        }
+        if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
+            const u4_t w = __builtin_bit_cast(u4_t, pf);
+            const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
+            pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
+        }
+        return pf;
     }
-    __device__ __forceinline__ void add(const Tile (&tile)[U], const Operand& w) {
+    __device__ __forceinline__ void add(const Tile& tile, const h8_t& w) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int T = 0; T < OT; ++T)
-                acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(tile[u].v[T / n], T % n), w.p[u], acc[T], 0, 0, 0);
-            if constexpr (CODES) {
-                const half_t one = (half_t)1.0f;
-                psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w.p[u], psum, 0, 0, 0);
-            }
+        for (int T = 0; T < OT; ++T)
+            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(tile.v[T / n], T % n), w, acc[T], 0, 0, 0);
+        if constexpr (CODES) {
+            const half_t one = (half_t)1.0f;
+            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w, psum, 0, 0, 0);
         }
     }
     // The sums as they stand: over the lane groups, and for codes the units, the codes' middle (taken off with the very
@@ -373,21 +346,18 @@ struct Flag {
     static constexpr bool value = V;
 };
 
-// Sums relative to a maximum, joined over NW waves: wave v adds up the output tiles T = v * OT / NW .. of all of them.
-template <int D, int KIND, int PACK>
+// Four waves' sums, each relative to its own reference: wave v adds up the output tiles T = v * D / 64 .. of all four.
+template <int D>
 struct PaJoin {
-    using W = PaWave<D, KIND, PACK>;
-    static constexpr int MINE = W::OT / 4;
     float m[4][16], l[4][16];
-    f4_t o[4][W::OT][64];
+    f4_t o[4][D / 16][64];
 };
 
-template <int D, int KIND, int PACK, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
+template <int D, int KIND, int PACK, int HT>
+__global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 256 ? 1 : 2) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
+    constexpr int NW = pa_waves(KIND), MINE = D / 64;
     using W = PaWave<D, KIND, PACK>;
-    using J = PaJoin<D, KIND, PACK>;
-    constexpr int MINE = J::MINE, U = W::U;
-    __shared__ J join;
+    __shared__ PaJoin<D> join;
     __shared__ int last;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int G = p.H / p.KV, run = blockIdx.x;
@@ -404,15 +374,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_at
         return v * sp.tasks_a_sequence;
     };
     // One workgroup a CU where the shares come out even or are long, else as many as there are.
-    constexpr int STEP = NW * U;                                           // tiles a workgroup takes at once
     const int units = sum_over([](int n) { return n; }), most = gridDim.x;
-    auto quota_of = [&](int units, int shares) { return (max((units + shares - 1) / shares, PA_MIN_STEPS * STEP) + STEP - 1) / STEP * STEP; };
-    auto pieces_of = [](int n, int q) { return n <= PA_MIN_STEPS * STEP * 3 / 2 ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
+    auto quota_of = [&](int units, int shares) { return (max((units + shares - 1) / shares, PA_MIN_STEPS * NW) + NW - 1) / NW * NW; };
+    auto pieces_of = [](int n, int q) { return n <= PA_MIN_STEPS * NW * 3 / 2 ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
     auto pieces = [&](int q) { return sum_over([&](int n) { return pieces_of(n, q); }); };
     int shares = min(most, 256), quota = quota_of(units, shares);
     bool even = pieces(quota) <= shares;
     for (int pass = 0; !even; ++pass) {
-        const int more = (quota + quota / 8 + STEP - 1) / STEP * STEP;
+        const int more = (quota + quota / 8 + NW - 1) / NW * NW;
         even = pieces(more) <= shares;
         if (even) {
             quota = more;
@@ -465,64 +434,56 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_at
             first_share = task0 / quota;
             parts = (task0 + seq.tiles - 1) / quota - first_share + 1;
         }
-        const int head = task / sp.head_tiles, h0 = (task - head * sp.head_tiles) * 16, used = min(16, G - h0);
+        const int head = task / sp.head_tiles, h0 = (task - head * sp.head_tiles) * 16 * HT, used = min(16 * HT, G - h0);
 
-        W w;
-        const int hcol = PACK == 2 ? col & 7 : col;                        // the column's query head
-        w.load_q(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(hcol, used - 1)) * D, hcol < used, g);
-        // this wave's steps: U neighbouring tiles each, from ta + U (wave + NW i); behind tb the last tile again, masked.  The
-        // tiles' places in the pool: 64 at a time, one a lane
-        const int count = (tb - ta - wave * U + NW * U - 1) / (NW * U);
-        const int hi = min(seq.hi, (seq.first + tb) * KV_TILE);
+        W w[HT];
+#pragma unroll
+        for (int x = 0; x < HT; ++x) {
+            const int hcol = (PACK == 2 ? col & 7 : col) + 16 * x;         // the column's query head
+            w[x].load_q(static_cast<const half_t*>(p.q) + b * p.q_batch + (size_t)(head * G + h0 + min(hcol, used - 1)) * D, hcol < used, g);
+        }
+        // this wave's tiles: ta + wave + NW i; their places in the pool: 64 at a time, one a lane
+        const int count = (tb - ta - wave + NW - 1) / NW;
         const char* cache = static_cast<const char*>(p.cache);
         int places = -1;
-        auto place_of = [&](int k) {                                       // of tile k of the wave
-            if ((k & 63) == 0) {
-                const int t = seq.first + min(ta + ((k + lane) / U * NW + wave) * U + (k + lane) % U, tb - 1);
-                const int page = t / p.page_tiles;
-                places = -1;
-                if (page < p.max_pages) {
-                    const int id = p.page_table[(size_t)b * p.max_pages + page];
-                    if (id >= 0 && id < p.num_pages) places = (id * p.KV + head) * p.page_tiles + t - page * p.page_tiles;
-                }
+        auto place_of = [&](int i) {
+            if ((i & 63) == 0) {
+                const int t = seq.first + min(ta + (i + lane) * NW + wave, tb - 1), page = t / p.page_tiles;
+                const int id = p.page_table[(size_t)b * p.max_pages + page];
+                places = id >= 0 && id < p.num_pages ? (id * p.KV + head) * p.page_tiles + t - page * p.page_tiles : -1;
             }
-            return __builtin_amdgcn_readlane(places, k & 63);
+            return __builtin_amdgcn_readlane(places, i & 63);
         };
-        // the registers of a step's keys, then of its values, are loaded for the next step as soon as they are used up
-        typename W::Tile tile[U];
-        int place[U];
+        // the registers of a tile's keys, then of its values, are loaded for the next tile as soon as they are used up
+        typename W::Tile tile;
+        int place = 0;
         auto fetch_keys = [&](int i) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                place[u] = place_of(i * U + u);
-                w.load_keys(tile[u], cache + (size_t)max(place[u], 0) * W::TILE_BYTES, lane);
-            }
+            place = place_of(i);
+            W::load_keys(tile, cache + (size_t)max(place, 0) * W::TILE_BYTES, lane);
         };
-        auto fetch_values = [&]() {
-#pragma unroll
-            for (int u = 0; u < U; ++u) w.load_values(tile[u], cache + (size_t)max(place[u], 0) * W::TILE_BYTES, lane);
-        };
+        auto fetch_values = [&]() { W::load_values(tile, cache + (size_t)max(place, 0) * W::TILE_BYTES, lane); };
         if (count > 0) {
             fetch_keys(0);
             fetch_values();
         }
-        w.start(col, sp.c);
+#pragma unroll
+        for (int x = 0; x < HT; ++x) w[x].start(col, sp.c);
         // (a load under a condition would make the compiler wait for every load wherever it waits for one)
         auto step = [&](auto more, int i) {
-            typename W::Scores sc[U];
-            typename W::Factors fac[U];
-            bool bad[U];
+            typename W::Scores sc[HT];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                sc[u] = w.scores(tile[u], lane);
-                fac[u] = tile[u].f;
-                bad[u] = place[u] < 0;
-            }
+            for (int x = 0; x < HT; ++x) sc[x] = w[x].scores(tile, lane);
+            typename W::Factors fac = tile.f;
+            const bool bad = place < 0;
             if constexpr (more.value) fetch_keys(i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            const typename W::Operand o = w.weights(sc, tile, fac, (seq.first + ta + (wave + NW * i) * U) * KV_TILE, seq.lo, hi, bad, lane);
+            h8_t o[HT];
+#pragma unroll
+            for (int x = 0; x < HT; ++x)
+                o[x] = w[x].weights(sc[x], tile, fac, (seq.first + ta + wave + NW * i) * KV_TILE, seq.lo, seq.hi, bad, lane);
             __builtin_amdgcn_sched_barrier(0);                 // values are decoded where they are used: not before, into registers
-            w.add(tile, o);
+#pragma unroll
+            for (int x = 0; x < HT; ++x) w[x].add(tile, o[x]);
             if constexpr (more.value) fetch_values();
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -531,57 +492,62 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_at
         if (i < count) step(Flag<false>(), i);
 
         // the waves' sums, joined
-        w.finish();
-#pragma unroll
-        for (int f = NW / 4 - 1; f >= 0; --f) {                // four waves at a time: the second four hand over to the first
-            if (wave / 4 == f) {
-                if (g == 0) { join.m[wave & 3][col] = w.m; join.l[wave & 3][col] = w.l; }
-#pragma unroll
-                for (int T = 0; T < W::OT; ++T) join.o[wave & 3][T][lane] = w.acc[T];
-            }
-            __syncthreads();
-            if (f > 0) {
-                if (wave / 4 == f - 1) {
-                    const float m1 = join.m[wave & 3][col], m2 = fmaxf(w.m, m1);
-                    const float a0 = __builtin_amdgcn_exp2f(w.m - m2), a1 = __builtin_amdgcn_exp2f(m1 - m2);
-                    w.l = w.l * a0 + join.l[wave & 3][col] * a1;
-                    w.m = m2;
-#pragma unroll
-                    for (int T = 0; T < W::OT; ++T) w.acc[T] = w.acc[T] * a0 + join.o[wave & 3][T][lane] * a1;
-                }
-                __syncthreads();
-            }
-        }
-        float mm = PA_NEG, ll = 0.0f, a[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mm = fmaxf(mm, join.m[v][col]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
-            ll += a[v] * join.l[v][col];
-        }
         const bool complete = parts == 1;
         float* slot = sp.partial + ((size_t)run * 2 + (ta == 0)) * sp.slot;
         half_t* out = out0 + ((size_t)b * p.H + head * G + h0) * D;
-        const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
-        if (wave < 4 && col < used) {
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const int T = wave * MINE + i;
-                f4_t o = {};
+        for (int x = 0; x < HT; ++x) {
+            w[x].finish();
+            if (x > 0) __syncthreads();                        // the arrays are written again
 #pragma unroll
-                for (int v = 0; v < 4; ++v) o = o + join.o[v][T][lane] * a[v];
+            for (int f = NW / 4 - 1; f >= 0; --f) {            // four waves at a time: the second four hand over to the first
+                if (wave / 4 == f) {
+                    if (g == 0) { join.m[wave & 3][col] = w[x].m; join.l[wave & 3][col] = w[x].l; }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = W::d_of(T, 4 * g + r);
-                    const float x = o[r];
-                    if (complete) out[(size_t)col * D + d] = (half_t)(x * norm);
-                    else __hip_atomic_store(slot + 32 + col * D + d, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    for (int T = 0; T < W::OT; ++T) join.o[wave & 3][T][lane] = w[x].acc[T];
+                }
+                __syncthreads();
+                if (f > 0) {
+                    if (wave / 4 == f - 1) {
+                        const float m1 = join.m[wave & 3][col], m2 = fmaxf(w[x].m, m1);
+                        const float a0 = __builtin_amdgcn_exp2f(w[x].m - m2), a1 = __builtin_amdgcn_exp2f(m1 - m2);
+                        w[x].l = w[x].l * a0 + join.l[wave & 3][col] * a1;
+                        w[x].m = m2;
+#pragma unroll
+                        for (int T = 0; T < W::OT; ++T) w[x].acc[T] = w[x].acc[T] * a0 + join.o[wave & 3][T][lane] * a1;
+                    }
+                    __syncthreads();
                 }
             }
-            if (!complete && wave == 0 && g == 0) {
-                __hip_atomic_store(slot + col, mm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(slot + 16 + col, ll, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            float mm = PA_NEG, ll = 0.0f, a[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) mm = fmaxf(mm, join.m[v][col]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
+                ll += a[v] * join.l[v][col];
+            }
+            const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
+            float* part = slot + x * (32 + 16 * D);
+            if (wave < 4 && col + 16 * x < used) {
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) {
+                    const int T = wave * MINE + i;
+                    f4_t o = {};
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) o = o + join.o[v][T][lane] * a[v];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = W::d_of(T, 4 * g + r);
+                        const float y = o[r];
+                        if (complete) out[(size_t)(col + 16 * x) * D + d] = (half_t)(y * norm);
+                        else __hip_atomic_store(part + 32 + col * D + d, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
+                }
+                if (!complete && wave == 0 && g == 0) {
+                    __hip_atomic_store(part + col, mm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(part + 16 + col, ll, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
             }
         }
         if (!complete) {
@@ -595,14 +561,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void paged_at
             if (last) {
                 auto slot_of = [&](int v) { return sp.partial + ((size_t)(w0 + v) * 2 + (v == 0)) * sp.slot; };
                 for (int i = threadIdx.x; i < used * D; i += 64 * NW) {
-                    const int hc = i / D;
+                    const int hc = i / D % 16, x = i / (16 * D);
                     float top = PA_NEG, sum = 0.0f, o = 0.0f;
 #pragma unroll 4
                     for (int v = 0; v < n; ++v) {
-                        const float* s = slot_of(v);
+                        const float* s = slot_of(v) + x * (32 + 16 * D);
                         const float mv = __hip_atomic_load(s + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         const float lv = __hip_atomic_load(s + 16 + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        const float ov = __hip_atomic_load(s + 32 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        const float ov = __hip_atomic_load(s + 32 + i % (16 * D), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         const float next = fmaxf(top, mv);
                         const float keep = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(mv - next);
                         sum = sum * keep + f * lv;
@@ -643,27 +609,30 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
         return kmi_set_error(KMI_E_SHAPE, "%s: need H a multiple of KV, window>=0 and a positive finite scale (H=%d KV=%d window=%d scale=%g)",
                              fn, p.H, p.KV, p.window, (double)p.scale);
     if (p.B == 0) return KMI_OK;
-    const int G = p.H / p.KV, used = G < 16 ? G : 16;
+    const long long pool = (long long)p.B * p.KV * p.max_pages * p.page_tiles;
+    const int G = p.H / p.KV, columns = G > 16 && p.D < 256 && pool >= PA_WIDE ? 32 : 16, used = G < columns ? G : columns;
     PaSplit sp;
-    sp.head_tiles = (G + 15) / 16;
+    sp.head_tiles = (G + columns - 1) / columns;
     sp.tasks_a_sequence = p.KV * sp.head_tiles;
     sp.c = p.scale * 1.44269504088896340736f;
-    sp.slot = 32 + used * p.D;
+    sp.slot = used > 16 ? 2 * (32 + 16 * p.D) : 32 + used * p.D;
     sp.counters = static_cast<uint32_t*>(p.workspace);
     sp.partial = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + KMI_GEMV_WS_HEADER);
-    // as many workgroups as the GPU holds at once, never more than the tasks can be cut into
-    const long long most = (long long)p.B * sp.tasks_a_sequence * p.max_pages * p.page_tiles;
-    if (most > 0x7FFFFFFFll)
+    // as many workgroups as the kernel may want, never more than the tasks can be cut into
+    const long long most = (long long)p.B * sp.tasks_a_sequence * ((long long)p.max_pages * p.page_tiles + PA_TASK_COST);
+    if (most > 0x7FFF0000ll)
         return kmi_set_error(KMI_E_SHAPE, "%s: %d sequences of %d pages hold more than 2^31 tiles", fn, p.B, p.max_pages);
     const long long pieces = (long long)p.B * sp.tasks_a_sequence * (((long long)p.max_pages * p.page_tiles + 7) / 8);
-    const int most_runs = PA_NW == 8 ? 256 : 512, runs = (int)(pieces < most_runs ? pieces : most_runs);
+    const int waves = pa_waves(p.kind), most_runs = waves == 8 ? 256 : 512, runs = (int)(pieces < most_runs ? pieces : most_runs);
     const size_t need = KMI_GEMV_WS_HEADER + (size_t)most_runs * 2 * sp.slot * sizeof(float);
     if (!p.workspace || p.workspace_bytes < need)
         return kmi_set_error(KMI_E_SHAPE, "%s: the workspace must hold %zu bytes (has %zu)", fn, need, p.workspace ? (size_t)p.workspace_bytes : (size_t)0);
-    const dim3 grid(runs), block(PA_NW * 64);
+    const dim3 grid(runs), block(waves * 64);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define KMI_PA_KIND(D_, K_) \
-    hipLaunchKernelGGL((G <= 8 && K_ != KMI_KV_F16 ? paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, PA_NW> : paged_attn_kernel<D_, K_, 1, PA_NW>), grid, block, 0, st, p, sp)
+#define KMI_PA_KIND(D_, K_)                                                                                                     \
+    if (columns == 32) hipLaunchKernelGGL((paged_attn_kernel<D_, K_, 1, D_ == 256 ? 1 : 2>), grid, block, 0, st, p, sp);        \
+    else if (G > 8 || K_ == KMI_KV_F16) hipLaunchKernelGGL((paged_attn_kernel<D_, K_, 1, 1>), grid, block, 0, st, p, sp);       \
+    else hipLaunchKernelGGL((paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, 1>), grid, block, 0, st, p, sp)
 #define KMI_PA_LAUNCH(D_)                                          \
     switch (p.kind) {                                              \
         case KMI_KV_F16: KMI_PA_KIND(D_, KMI_KV_F16); break;       \
