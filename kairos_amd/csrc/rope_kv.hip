@@ -65,65 +65,84 @@ __device__ __forceinline__ int code_of(float x, float z, float r, float lo, floa
     return (int)fminf(fmaxf(rintf((x - z) * r), lo), hi);      // the clamp also turns a NaN into a number
 }
 
-// Codes of eight elements: int8 two words of four bytes, int4 element e in nibble e / 2 + 4 (e % 2) of one word.
+// Eight elements of a row as the cache holds them: elements, or codes (bytes; nibbles), in order.  NPW = 32-bit words.
 template <int KIND>
-__device__ __forceinline__ void row_codes(h8_t x, const RowFactors& f, int (&u)[8]) {
+struct Packed {
+    static constexpr int NPW = 4 / kv_per_word(KIND);
+    uint32_t w[NPW];
+};
+template <int KIND>
+__device__ __forceinline__ Packed<KIND> pack_row(h8_t x, const RowFactors& f) {
+    Packed<KIND> o;
+    if constexpr (KIND == KMI_KV_F16) {
+        const u4_t w = __builtin_bit_cast(u4_t, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if constexpr (KIND == KMI_KV_INT8) u[e] = code_of((float)x[e], 0.0f, f.r, -127.0f, 127.0f) + 128;
-        else u[e] = code_of((float)x[e], (float)f.z, f.r, 0.0f, 15.0f);
+        for (int i = 0; i < 4; ++i) o.w[i] = w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < Packed<KIND>::NPW; ++i) o.w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (KIND == KMI_KV_INT8) o.w[e / 4] |= (uint32_t)(code_of((float)x[e], 0.0f, f.r, -127.0f, 127.0f) + 128) << (8 * (e % 4));
+            else o.w[0] |= (uint32_t)code_of((float)x[e], (float)f.z, f.r, 0.0f, 15.0f) << (4 * e);
+        }
+    }
+    return o;
+}
+// Nibble e of a key unit stands at place e / 2 + 4 (e % 2): even elements in the low half, odd ones in the high.
+__device__ __forceinline__ uint32_t nibbles_apart(uint32_t w) {
+    uint32_t e = w & 0x0F0F0F0Fu, o = (w >> 4) & 0x0F0F0F0Fu;
+    e = (e | e >> 4) & 0x00FF00FFu; e = (e | e >> 8) & 0xFFFFu;
+    o = (o | o >> 4) & 0x00FF00FFu; o = (o | o >> 8) & 0xFFFFu;
+    return e | o << 16;
+}
+__device__ __forceinline__ uint32_t nibbles_together(uint32_t w) {
+    uint32_t e = w & 0xFFFFu, o = w >> 16;
+    e = (e | e << 8) & 0x00FF00FFu; e = (e | e << 4) & 0x0F0F0F0Fu;
+    o = (o | o << 8) & 0x00FF00FFu; o = (o | o << 4) & 0x0F0F0F0Fu;
+    return e | o << 4;
+}
+
+template <int D, int KIND>
+__device__ __forceinline__ void store_factors(char* tile, int tau, int d0, int first, const RowFactors& f) {
+    if constexpr (KIND != KMI_KV_F16) {
+        if (d0 != 0) return;
+        *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first)) = f.s;
+        if constexpr (KIND == KMI_KV_INT4) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first + 1)) = f.z;
     }
 }
 
 template <int D, int KIND>
 __device__ __forceinline__ void store_key(char* tile, int tau, int d0, h8_t x) {
+    RowFactors f = {};
+    if constexpr (KIND != KMI_KV_F16) f = row_factors<D / 8, KIND>(x);
+    const Packed<KIND> w = pack_row<KIND>(x, f);
     char* at = tile + kv_key_offset<D, KIND>(tau, d0);
-    if constexpr (KIND == KMI_KV_F16) {
-        *reinterpret_cast<h8_t*>(at) = x;
-    } else {
-        const RowFactors f = row_factors<D / 8, KIND>(x);
-        int u[8];
-        row_codes<KIND>(x, f, u);
-        if constexpr (KIND == KMI_KV_INT8) {
-            u2_t w;
-            w[0] = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
-            w[1] = u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24;
-            *reinterpret_cast<u2_t*>(at) = w;
-        } else {
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w |= (uint32_t)u[e] << (4 * (e / 2 + 4 * (e & 1)));
-            *reinterpret_cast<uint32_t*>(at) = w;
-        }
-        if (d0 == 0) {
-            *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, 0)) = f.s;
-            if constexpr (KIND == KMI_KV_INT4) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, 1)) = f.z;
-        }
-    }
+    if constexpr (KIND == KMI_KV_F16) *reinterpret_cast<u4_t*>(at) = u4_t{w.w[0], w.w[1], w.w[2], w.w[3]};
+    else if constexpr (KIND == KMI_KV_INT8) *reinterpret_cast<u2_t*>(at) = u2_t{w.w[0], w.w[1]};
+    else *reinterpret_cast<uint32_t*>(at) = nibbles_apart(w.w[0]);
+    store_factors<D, KIND>(tile, tau, d0, 0, f);
 }
 
+// One token's value: its words stand 16 bytes apart.
 template <int D, int KIND>
-__device__ __forceinline__ void store_value(char* tile, int tau, int d0, h8_t x) {
-    if constexpr (KIND == KMI_KV_F16) {
+__device__ __forceinline__ void store_value(char* tile, int tau, int d0, const Packed<KIND>& w) {
+    constexpr int n = kv_per_word(KIND);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) *reinterpret_cast<half_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + e)) = x[e];
-    } else {
-        const RowFactors f = row_factors<D / 8, KIND>(x);
-        int u[8];
-        row_codes<KIND>(x, f, u);
-        constexpr int n = kv_per_word(KIND);
+    for (int i = 0; i < 8 / n; ++i)
+        *reinterpret_cast<uint16_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + n * i)) = (uint16_t)(w.w[i / 2] >> (16 * (i & 1)));
+}
+// Eight tokens tau0 .. tau0 + 7 (tau0 % 8 == 0): whole 16-byte chunks, 128 / n bytes in a row.
+template <int D, int KIND>
+__device__ __forceinline__ void store_values8(char* tile, int tau0, int d0, const Packed<KIND> (&w)[8]) {
+    constexpr int n = kv_per_word(KIND);
+    u4_t* at = reinterpret_cast<u4_t*>(tile + kv_value_offset<D, KIND>(tau0, d0));
 #pragma unroll
-        for (int w = 0; w < 8 / n; ++w) {
-            int bits = 0;
+    for (int i = 0; i < 8 / n; ++i) {
+        u4_t c;
 #pragma unroll
-            for (int a = 0; a < n; ++a) bits |= u[n * w + a] << (16 / n * a);
-            *reinterpret_cast<uint16_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + n * w)) = (uint16_t)bits;
-        }
-        if (d0 == 0) {
-            constexpr int i = kv_factors(KIND) / 2;
-            *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, i)) = f.s;
-            if constexpr (KIND == KMI_KV_INT4) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, 3)) = f.z;
-        }
+        for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_perm(w[2 * j + 1].w[i / 2], w[2 * j].w[i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+        at[i] = c;
     }
 }
 
@@ -145,8 +164,8 @@ struct Angles {
             c[2 * i + 1] = inside ? v[2] : nan; s[2 * i + 1] = inside ? v[3] : nan;
         }
     }
-    // x: the lane's elements; row: the row's first element (for the partner of the half layout)
-    __device__ __forceinline__ h8_t turn(h8_t x, const half_t* row, int R, int d0) const {
+    // x: the lane's elements; o: their partners (half layout)
+    __device__ __forceinline__ h8_t turn(h8_t x, h8_t o, int R, int d0) const {
 #pragma clang fp contract(off)
         if (d0 >= R) return x;
         h8_t y;
@@ -159,7 +178,6 @@ struct Angles {
             }
         } else {
             const bool first = d0 < R / 2;
-            const h8_t o = *reinterpret_cast<const h8_t*>(row + (first ? d0 + R / 2 : d0 - R / 2));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float a = (float)x[e], b = (float)o[e];
@@ -171,47 +189,95 @@ struct Angles {
     }
 };
 
-// One workgroup: `span` neighbouring tokens of one sequence, all their rows (queries, keys, values), eight elements a lane.
-// A lane keeps the angles of its elements for all rows of a token.
+// One workgroup: eight neighbouring positions 8 i .. 8 i + 7 of one sequence, 2048 / D rows (heads of queries, keys or values) of each;
+// a lane has eight elements of one row.  Where all eight tokens are there, all loads are in flight before the first use,
+// and the values leave as whole chunks of the cache, turned over in registers.
 template <int D, int KIND, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p, int span) {
-    constexpr int LPR = D / 8, ROWS = 256 / LPR;
-    constexpr int TILE_BYTES = KIND < 0 ? 0 : kv_tile_bytes(D, KIND < 0 ? 0 : KIND);
-    const int b = blockIdx.y;
-    const int d0 = (threadIdx.x % LPR) * 8, r0 = threadIdx.x / LPR;
+__global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
+    constexpr int LPR = D / 8, ROWS = 256 / LPR, K_ = KIND < 0 ? 0 : KIND;
+    const int b = blockIdx.y, d0 = (threadIdx.x % LPR) * 8, R = p.rotary_dim;
+    const int r = (p.q ? 0 : p.H) + blockIdx.z * ROWS + threadIdx.x / LPR;
+    if (r >= p.H + p.KV + (KIND >= 0 ? p.KV : 0)) return;
+    const bool is_q = r < p.H, is_v = r >= p.H + p.KV;
+    const int head = is_q ? r : is_v ? r - p.H - p.KV : r - p.H;
     const int start = p.start[b], count = p.count ? min(p.count[b], p.S) : p.S;
-    const int first = p.q ? 0 : p.H, rows = p.H + p.KV + (KIND >= 0 ? p.KV : 0);
+    const int pos0 = (int)((unsigned)((start >> 3) + (int)blockIdx.x) << 3), s0 = (int)((unsigned)pos0 - (unsigned)start);
+    if (s0 >= p.S) return;
+
+    const int heads = is_q ? p.H : p.KV;
+    const half_t* row = is_q ? static_cast<const half_t*>(p.q) + b * p.q_batch : is_v ? static_cast<const half_t*>(p.v) + b * p.v_batch
+                                                                                     : static_cast<const half_t*>(p.k) + b * p.k_batch;
+    const int64_t step = is_q ? p.q_token : is_v ? p.v_token : p.k_token;
+    row += (size_t)head * D;
+    half_t* out = static_cast<half_t*>(is_q ? p.q_out : is_v ? nullptr : p.k_out);
+    if (out) out += ((size_t)b * p.S * heads + head) * D + d0;
+    const size_t out_step = (size_t)heads * D;
     const KvPlace place = {static_cast<char*>(p.cache), p.page_table, p.num_pages, p.page_tiles, p.max_pages, p.KV};
-    half_t* q_out = static_cast<half_t*>(p.q_out);
-    half_t* k_out = static_cast<half_t*>(p.k_out);
+    char* tile = nullptr;                                       // the eight positions lie in one tile
+    if constexpr (KIND >= 0) tile = is_q || pos0 < 0 ? nullptr : kv_tile_at<kv_tile_bytes(D, K_)>(place, b, head, pos0 / KV_TILE);
+    const int tau0 = pos0 & (KV_TILE - 1);
+    const int partner = INTERLEAVED || d0 >= R ? d0 : d0 < R / 2 ? d0 + R / 2 : d0 - R / 2;
+    const float* table = static_cast<const float*>(p.table);
     Angles<INTERLEAVED> ang;
-    for (int s = blockIdx.x * span; s < min((int)(blockIdx.x + 1) * span, p.S); ++s) {
-        const bool valid = s < count;
-        const int pos = valid ? (int)((unsigned)start + (unsigned)s) : 0;
-        if (valid) ang.load(static_cast<const float*>(p.table), p.table_rows, p.rotary_dim, pos, d0);
-        const size_t token = (size_t)b * p.S + s;
-        for (int r = first + r0; r < rows; r += ROWS) {
-            const bool is_q = r < p.H, is_k = !is_q && r < p.H + p.KV;
-            const int head = is_q ? r : is_k ? r - p.H : r - p.H - p.KV;
-            half_t* out = is_q ? q_out + (token * p.H + head) * D : is_k && k_out ? k_out + (token * p.KV + head) * D : nullptr;
-            if (!valid) {                                       // rows behind the sequence: zeros out, nothing into the cache
-                if (out) *reinterpret_cast<h8_t*>(out + d0) = h8_t{};
-                continue;
-            }
-            const half_t* row = is_q ? static_cast<const half_t*>(p.q) + b * p.q_batch + s * p.q_token
-                              : is_k ? static_cast<const half_t*>(p.k) + b * p.k_batch + s * p.k_token
-                                     : static_cast<const half_t*>(p.v) + b * p.v_batch + s * p.v_token;
-            row += (size_t)head * D;
-            h8_t x = *reinterpret_cast<const h8_t*>(row + d0);
-            if (is_q || is_k) x = ang.turn(x, row, p.rotary_dim, d0);
-            if (out) *reinterpret_cast<h8_t*>(out + d0) = x;
+
+    if (s0 >= 0 && s0 + 8 <= count) {
+        h8_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const h8_t*>(row + (s0 + j) * step + d0);
+        if (is_v) {
             if constexpr (KIND >= 0) {
-                if (is_q) continue;
-                // the lanes of a row go together: the row's factors are joined over them
-                char* tile = pos < 0 ? nullptr : kv_tile_at<TILE_BYTES>(place, b, head, pos / KV_TILE);
-                if (!tile) continue;
-                if (is_k) store_key<D, KIND>(tile, pos % KV_TILE, d0, x);
-                else store_value<D, KIND>(tile, pos % KV_TILE, d0, x);
+                if (!tile) return;
+                Packed<K_> w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    RowFactors f = {};
+                    if constexpr (K_ != KMI_KV_F16) f = row_factors<LPR, K_>(x[j]);
+                    w[j] = pack_row<K_>(x[j], f);
+                    store_factors<D, K_>(tile, tau0 + j, d0, kv_factors(K_) / 2, f);
+                }
+                store_values8<D, K_>(tile, tau0, d0, w);
+            }
+            return;
+        }
+        h8_t o[8];
+        if constexpr (!INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = *reinterpret_cast<const h8_t*>(row + (s0 + j) * step + partner);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            ang.load(table, p.table_rows, R, pos0 + j, d0);
+            const h8_t y = ang.turn(x[j], INTERLEAVED ? x[j] : o[j], R, d0);
+            if (out) *reinterpret_cast<h8_t*>(out + (s0 + j) * out_step) = y;
+            if constexpr (KIND >= 0) {
+                if (tile) store_key<D, K_>(tile, tau0 + j, d0, y);
+            }
+        }
+        return;
+    }
+    for (int j = 0; j < 8; ++j) {
+        const int s = s0 + j;
+        if (s < 0 || s >= p.S) continue;
+        if (s >= count) {                                       // rows behind the sequence: zeros out, nothing into the cache
+            if (out) *reinterpret_cast<h8_t*>(out + s * out_step) = h8_t{};
+            continue;
+        }
+        h8_t x = *reinterpret_cast<const h8_t*>(row + s * step + d0);
+        if (!is_v) {
+            const h8_t o = *reinterpret_cast<const h8_t*>(row + s * step + partner);
+            ang.load(table, p.table_rows, R, pos0 + j, d0);
+            x = ang.turn(x, o, R, d0);
+        }
+        if (out) *reinterpret_cast<h8_t*>(out + s * out_step) = x;
+        if constexpr (KIND >= 0) {
+            if (!tile) continue;
+            if (is_v) {
+                RowFactors f = {};
+                if constexpr (K_ != KMI_KV_F16) f = row_factors<LPR, K_>(x);
+                store_value<D, K_>(tile, tau0 + j, d0, pack_row<K_>(x, f));
+                store_factors<D, K_>(tile, tau0 + j, d0, kv_factors(K_) / 2, f);
+            } else {
+                store_key<D, K_>(tile, tau0 + j, d0, x);
             }
         }
     }
@@ -224,55 +290,86 @@ __device__ __forceinline__ half_t value_of(int u, float s, float z) {
     return (half_t)(v > 65504.0f ? 65504.0f : v < -65504.0f ? -65504.0f : v);
 }
 
-// Eight elements a lane of one token of one head, keys and values.
+// Eight packed elements to fp16.
+template <int KIND>
+__device__ __forceinline__ h8_t unpack_row(const Packed<KIND>& w, float s, float z) {
+    if constexpr (KIND == KMI_KV_F16) {
+        return __builtin_bit_cast(h8_t, u4_t{w.w[0], w.w[1], w.w[2], w.w[3]});
+    } else {
+        h8_t o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (KIND == KMI_KV_INT8) o[e] = value_of<KIND>((w.w[e / 4] >> (8 * (e % 4))) & 255, s, 0.0f);
+            else o[e] = value_of<KIND>((w.w[0] >> (4 * e)) & 15, s, z);
+        }
+        return o;
+    }
+}
+
+// One workgroup: eight neighbouring positions 8 i .. 8 i + 7 of one sequence, 2048 / D rows (key heads, then value heads); a lane
+// reads eight elements of one row of all eight tokens (whole chunks of values, turned over in registers).
 template <int D, int KIND>
 __global__ __launch_bounds__(256) void kv_read_kernel(kmi_kv_read_args p) {
-    constexpr int LPR = D / 8, n = kv_per_word(KIND);
-    const int b = blockIdx.y;
-    const long item = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;       // (token, head)
-    if (item >= (long)p.S * p.KV) return;
-    const int s = (int)(item / p.KV), head = (int)(item - (long)s * p.KV), d0 = (threadIdx.x % LPR) * 8;
-    const size_t at = (((size_t)b * p.S + s) * p.KV + head) * D + d0;
-    h8_t k = {}, v = {};
-    const int count = p.count ? p.count[b] : p.S;
-    if (s < count) {
-        const KvPlace place = {static_cast<char*>(const_cast<void*>(p.cache)), p.page_table, p.num_pages, p.page_tiles, p.max_pages, p.KV};
-        const int pos = (int)((unsigned)p.start[b] + (unsigned)s), tau = pos & (KV_TILE - 1);
-        const char* tile = pos < 0 ? nullptr : kv_tile_at<kv_tile_bytes(D, KIND)>(place, b, head, pos / KV_TILE);
-        if (!tile) {
-            const half_t nan = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
-            k = h8_t{nan, nan, nan, nan, nan, nan, nan, nan};
-            v = k;
-        } else if constexpr (KIND == KMI_KV_F16) {
-            k = *reinterpret_cast<const h8_t*>(tile + kv_key_offset<D, KIND>(tau, d0));
+    constexpr int LPR = D / 8, ROWS = 256 / LPR, n = kv_per_word(KIND), NF = kv_factors(KIND);
+    const int b = blockIdx.y, d0 = (threadIdx.x % LPR) * 8;
+    const int r = blockIdx.z * ROWS + threadIdx.x / LPR;
+    if (r >= 2 * p.KV) return;
+    const bool is_v = r >= p.KV;
+    const int head = is_v ? r - p.KV : r;
+    const int start = p.start[b], count = p.count ? min(p.count[b], p.S) : p.S;
+    const int pos0 = (int)((unsigned)((start >> 3) + (int)blockIdx.x) << 3), s0 = (int)((unsigned)pos0 - (unsigned)start);
+    if (s0 >= p.S) return;
+    half_t* out = static_cast<half_t*>(is_v ? p.v_out : p.k_out) + ((size_t)b * p.S * p.KV + head) * D + d0;
+    const size_t out_step = (size_t)p.KV * D;
+    const KvPlace place = {static_cast<char*>(const_cast<void*>(p.cache)), p.page_table, p.num_pages, p.page_tiles, p.max_pages, p.KV};
+    const char* tile = pos0 < 0 ? nullptr : kv_tile_at<kv_tile_bytes(D, KIND)>(place, b, head, pos0 / KV_TILE);
+    const int tau0 = pos0 & (KV_TILE - 1);
+
+    Packed<KIND> w[8] = {};
+    h8_t fs = {}, fz = {};                                      // scales and offsets of the eight tokens
+    if (tile) {
+        if constexpr (NF > 0) {
+            const int first = is_v ? NF / 2 : 0;
+            fs = *reinterpret_cast<const h8_t*>(tile + kv_factor_offset<D, KIND>(tau0, first));
+            if constexpr (NF == 4) fz = *reinterpret_cast<const h8_t*>(tile + kv_factor_offset<D, KIND>(tau0, first + 1));
+        }
+        if (is_v) {
+            const u4_t* at = reinterpret_cast<const u4_t*>(tile + kv_value_offset<D, KIND>(tau0, d0));
+            u4_t c[8 / n];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const half_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + e));
+            for (int i = 0; i < 8 / n; ++i) c[i] = at[i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int k = 0; k < Packed<KIND>::NPW; ++k)
+                    w[j].w[k] = __builtin_amdgcn_perm(c[2 * k + 1][j / 2], c[2 * k][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
         } else {
-            float f[4] = {};
 #pragma unroll
-            for (int i = 0; i < kv_factors(KIND); ++i) f[i] = (float)*reinterpret_cast<const half_t*>(tile + kv_factor_offset<D, KIND>(tau, i));
-            const char* kp = tile + kv_key_offset<D, KIND>(tau, d0);
-            if constexpr (KIND == KMI_KV_INT8) {
-                const u2_t w = *reinterpret_cast<const u2_t*>(kp);
+            for (int j = 0; j < 8; ++j) {
+                const char* at = tile + kv_key_offset<D, KIND>(tau0 + j, d0);
+                if constexpr (KIND == KMI_KV_F16) {
+                    const u4_t v = *reinterpret_cast<const u4_t*>(at);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) k[e] = value_of<KIND>((w[e / 4] >> (8 * (e % 4))) & 255, f[0], 0.0f);
-            } else {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(kp);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) k[e] = value_of<KIND>((w >> (4 * (e / 2 + 4 * (e & 1)))) & 15, f[0], f[1]);
-            }
-#pragma unroll
-            for (int w = 0; w < 8 / n; ++w) {
-                const int bits = *reinterpret_cast<const uint16_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + n * w));
-#pragma unroll
-                for (int a = 0; a < n; ++a)
-                    v[n * w + a] = value_of<KIND>((bits >> (16 / n * a)) & (KIND == KMI_KV_INT8 ? 255 : 15),
-                                                  KIND == KMI_KV_INT8 ? f[1] : f[2], f[3]);
+                    for (int k = 0; k < 4; ++k) w[j].w[k] = v[k];
+                } else if constexpr (KIND == KMI_KV_INT8) {
+                    const u2_t v = *reinterpret_cast<const u2_t*>(at);
+                    w[j].w[0] = v[0]; w[j].w[1] = v[1];
+                } else {
+                    w[j].w[0] = nibbles_together(*reinterpret_cast<const uint32_t*>(at));
+                }
             }
         }
     }
-    *reinterpret_cast<h8_t*>(static_cast<half_t*>(p.k_out) + at) = k;
-    *reinterpret_cast<h8_t*>(static_cast<half_t*>(p.v_out) + at) = v;
+    const half_t nan = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int s = s0 + j;
+        if (s < 0 || s >= p.S) continue;
+        h8_t x = unpack_row<KIND>(w[j], (float)fs[j], (float)fz[j]);
+        if (!tile) x = h8_t{nan, nan, nan, nan, nan, nan, nan, nan};
+        if (s >= count) x = h8_t{};
+        *reinterpret_cast<h8_t*>(out + s * out_step) = x;
+    }
 }
 
 // ---- C entries ---------------------------------------------------------------------------------------------------------
@@ -320,12 +417,12 @@ extern "C" int kmi_rope_kv(const kmi_rope_kv_args* args, void* stream) {
         if (rc < 0) return rc;
     }
     if (p.B == 0 || p.S == 0) return KMI_OK;
-    const int span = p.S >= 64 ? 8 : 1;
-    const dim3 grid((p.S + span - 1) / span, p.B), block(256);
+    const int rows = (p.q ? p.H : 0) + p.KV + (cached ? p.KV : 0), at_once = 2048 / p.D;
+    const dim3 grid((unsigned)(((long long)p.S + 14) / 8), p.B, (rows + at_once - 1) / at_once), block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int kind = cached ? p.kind : -1;
 #define KMI_ROPE_LAUNCH(D_, K_) \
-    hipLaunchKernelGGL((p.interleaved ? rope_kv_kernel<D_, K_, true> : rope_kv_kernel<D_, K_, false>), grid, block, 0, st, p, span)
+    hipLaunchKernelGGL((p.interleaved ? rope_kv_kernel<D_, K_, true> : rope_kv_kernel<D_, K_, false>), grid, block, 0, st, p)
 #define KMI_ROPE_KIND(D_)                                                                                             \
     switch (kind) {                                                                                                   \
         case KMI_KV_F16: KMI_ROPE_LAUNCH(D_, KMI_KV_F16); break;                                                      \
@@ -351,9 +448,9 @@ extern "C" int kmi_kv_read(const kmi_kv_read_args* args, void* stream) {
     if (rc < 0) return rc;
     if (p.S < 0) return kmi_set_error(KMI_E_SHAPE, "%s: need S>=0 (S=%d)", fn, p.S);
     if (p.B == 0 || p.S == 0) return KMI_OK;
-    const long per = 256 / (p.D / 8), blocks = ((long)p.S * p.KV + per - 1) / per;
-    if (blocks > 0x7FFFFFFF) return kmi_set_error(KMI_E_SHAPE, "%s: S * KV is too large (S=%d KV=%d)", fn, p.S, p.KV);
-    const dim3 grid((unsigned)blocks, p.B), block(256);
+    const int at_once = 2048 / p.D;
+    if (p.KV > 32767) return kmi_set_error(KMI_E_SHAPE, "%s: need KV<=32767 (KV=%d)", fn, p.KV);
+    const dim3 grid((unsigned)(((long long)p.S + 14) / 8), p.B, (2 * p.KV + at_once - 1) / at_once), block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define KMI_READ_LAUNCH(D_)                                                                                           \
     switch (p.kind) {                                                                                                 \
