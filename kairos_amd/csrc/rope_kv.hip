@@ -11,6 +11,7 @@
 // once: the codes are the same on any machine.  A row with an infinity or NaN gets the scale NaN and reads as NaN.
 // Traffic: every row read once and written once, plus the table's R * 4 bytes a token; a memory-bound kernel.
 #include "kv_parts.h"
+#include <type_traits>
 
 struct RowFactors {
     half_t s, z;
@@ -23,49 +24,60 @@ __device__ __forceinline__ half_t scale_up(float width, float steps) {
     return s;
 }
 
-// Factors of a row spread over LPR neighbouring lanes, eight elements each.
+typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+
+// v joined by f over LPR neighbouring lanes (4, 8 or 16), in all of them.
+template <int LPR, typename T, typename F>
+__device__ __forceinline__ T over_row(T v, F f) {
+    auto step = [&](auto ctrl) {
+        const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl.value, 0xF, 0xF, false);
+        v = f(v, __builtin_bit_cast(T, o));
+    };
+    step(std::integral_constant<int, 0xB1>());                 // quad_perm 1 0 3 2
+    step(std::integral_constant<int, 0x4E>());                 // quad_perm 2 3 0 1
+    if constexpr (LPR >= 8) step(std::integral_constant<int, 0x141>());       // row_half_mirror: the other four of eight
+    if constexpr (LPR >= 16) step(std::integral_constant<int, 0x140>());      // row_mirror: the other eight of sixteen
+    return v;
+}
+
+// Factors of a row spread over LPR neighbouring lanes, two chunks of eight elements each.
 template <int LPR, int KIND>
-__device__ __forceinline__ RowFactors row_factors(h8_t x) {
+__device__ __forceinline__ RowFactors row_factors(h8_t a, h8_t b) {
 #pragma clang fp contract(off)
-    int top = 0;                                        // largest |x| as bits: orders infinities and NaN above all
-    half_t lo = x[0], hi = x[0];
+    RowFactors f = {};
+    if constexpr (KIND == KMI_KV_F16) return f;
+    const u4_t wa = __builtin_bit_cast(u4_t, a), wb = __builtin_bit_cast(u4_t, b);
+    us2_t top = {};                                     // largest |x| as bits: orders infinities and NaN above all
+    h2_t lo = as_h2(wa[0]), hi = lo;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const half_t v = x[e];                          // a copy: a bit cast of a vector's element reads element 0
-        const int bits = __builtin_bit_cast(uint16_t, v) & 0x7FFF;
-        top = bits > top ? bits : top;
-        lo = x[e] < lo ? x[e] : lo;
-        hi = x[e] > hi ? x[e] : hi;
-    }
-    float flo = (float)lo, fhi = (float)hi;
-#pragma unroll
-    for (int off = LPR / 2; off > 0; off >>= 1) {
-        const int t = __shfl_xor(top, off, 64);
-        top = t > top ? t : top;
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w = i < 4 ? wa[i & 3] : wb[i & 3];
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(us2_t, w & 0x7FFF7FFFu));
         if constexpr (KIND == KMI_KV_INT4) {
-            flo = fminf(flo, __shfl_xor(flo, off, 64));
-            fhi = fmaxf(fhi, __shfl_xor(fhi, off, 64));
+            lo = __builtin_elementwise_min(lo, as_h2(w));
+            hi = __builtin_elementwise_max(hi, as_h2(w));
         }
     }
-    RowFactors f;
-    f.z = (half_t)0.0f;
+    top = over_row<LPR>(top, [](us2_t x, us2_t y) { return __builtin_elementwise_max(x, y); });
+    const uint16_t most = top[0] > top[1] ? top[0] : top[1];
     if constexpr (KIND == KMI_KV_INT8) {
-        f.s = scale_up((float)__builtin_bit_cast(half_t, (uint16_t)top), 127.0f);
+        f.s = scale_up((float)__builtin_bit_cast(half_t, most), 127.0f);
     } else {
-        f.z = (half_t)(flo + 0.0f);                     // never -0: which of two zeros is the smallest is left open
-        f.s = scale_up(fhi - flo, 15.0f);
+        const half_t l = lo[0] < lo[1] ? lo[0] : lo[1], h = hi[0] > hi[1] ? hi[0] : hi[1];
+        h2_t ends = {l, -h};
+        ends = over_row<LPR>(ends, [](h2_t x, h2_t y) { return __builtin_elementwise_min(x, y); });
+        const float flo = (float)ends[0] + 0.0f;        // never -0: which of two zeros is the smallest is left open
+        f.z = (half_t)flo;
+        f.s = scale_up(-(float)ends[1] - flo, 15.0f);
     }
-    if (top >= 0x7C00) f.s = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
+    if (most >= 0x7C00) f.s = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
     f.r = (float)f.s > 0.0f ? 1.0f / (float)f.s : 0.0f;
     return f;
 }
 
-__device__ __forceinline__ int code_of(float x, float z, float r, float lo, float hi) {
-#pragma clang fp contract(off)
-    return (int)fminf(fmaxf(rintf((x - z) * r), lo), hi);      // the clamp also turns a NaN into a number
-}
-
 // Eight elements of a row as the cache holds them: elements, or codes (bytes; nibbles), in order.  NPW = 32-bit words.
+// A code is rounded by adding 1.5 * 2^23 (+ 128): its bits are then the low ones of the sum, the others a constant that is taken
+// off the packed word once.  up() leaves no code outside its range, so nothing is clamped.
 template <int KIND>
 struct Packed {
     static constexpr int NPW = 4 / kv_per_word(KIND);
@@ -73,21 +85,58 @@ struct Packed {
 };
 template <int KIND>
 __device__ __forceinline__ Packed<KIND> pack_row(h8_t x, const RowFactors& f) {
+#pragma clang fp contract(off)
     Packed<KIND> o;
     if constexpr (KIND == KMI_KV_F16) {
         const u4_t w = __builtin_bit_cast(u4_t, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o.w[i] = w[i];
     } else {
+        constexpr int bits = KIND == KMI_KV_INT8 ? 8 : 4, per = 32 / bits;
+        constexpr uint32_t base = 0x4B400000u;          // of 1.5 * 2^23
 #pragma unroll
-        for (int i = 0; i < Packed<KIND>::NPW; ++i) o.w[i] = 0;
+        for (int i = 0; i < Packed<KIND>::NPW; ++i) {
+            uint32_t w = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (KIND == KMI_KV_INT8) o.w[e / 4] |= (uint32_t)(code_of((float)x[e], 0.0f, f.r, -127.0f, 127.0f) + 128) << (8 * (e % 4));
-            else o.w[0] |= (uint32_t)code_of((float)x[e], (float)f.z, f.r, 0.0f, 15.0f) << (4 * e);
+            for (int e = 0; e < per; ++e) {
+                const float v = KIND == KMI_KV_INT8 ? (float)x[per * i + e] * f.r + 12583040.0f
+                                                    : ((float)x[per * i + e] - (float)f.z) * f.r + 12582912.0f;
+                w += (__builtin_bit_cast(uint32_t, v)) << (bits * e);
+            }
+            uint32_t off = 0;
+#pragma unroll
+            for (int e = 0; e < per; ++e) off += base << (bits * e);
+            o.w[i] = w - off;
         }
     }
     return o;
+}
+// Four items of four lanes (a quad) turned over: item i of lane k becomes item k of lane i.
+template <typename T>
+__device__ __forceinline__ void turn_quad(T (&x)[4], int lane) {
+    constexpr int N = sizeof(T) / 4;
+    struct Words {
+        uint32_t w[N];
+    };
+    Words v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(Words, x[i]);
+    auto swap = [&](auto ctrl, int i, int j, bool upper) {     // item j of the lower lanes with item i of the upper ones
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t give = upper ? v[i].w[n] : v[j].w[n];
+            const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, ctrl.value, 0xF, 0xF, false);
+            v[i].w[n] = upper ? got : v[i].w[n];
+            v[j].w[n] = upper ? v[j].w[n] : got;
+        }
+    };
+    const bool odd = lane & 1, high = lane & 2;
+    swap(std::integral_constant<int, 0xB1>(), 0, 1, odd);
+    swap(std::integral_constant<int, 0xB1>(), 2, 3, odd);
+    swap(std::integral_constant<int, 0x4E>(), 0, 2, high);
+    swap(std::integral_constant<int, 0x4E>(), 1, 3, high);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(T, v[i]);
 }
 // Nibble e of a key unit stands at place e / 2 + 4 (e % 2): even elements in the low half, odd ones in the high.
 __device__ __forceinline__ uint32_t nibbles_apart(uint32_t w) {
@@ -104,24 +153,17 @@ __device__ __forceinline__ uint32_t nibbles_together(uint32_t w) {
 }
 
 template <int D, int KIND>
-__device__ __forceinline__ void store_factors(char* tile, int tau, int d0, int first, const RowFactors& f) {
-    if constexpr (KIND != KMI_KV_F16) {
-        if (d0 != 0) return;
-        *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first)) = f.s;
-        if constexpr (KIND == KMI_KV_INT4) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first + 1)) = f.z;
-    }
+__device__ __forceinline__ void store_factors(char* tile, int tau, int first, const RowFactors& f) {
+    if constexpr (KIND != KMI_KV_F16) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first)) = f.s;
+    if constexpr (KIND == KMI_KV_INT4) *reinterpret_cast<half_t*>(tile + kv_factor_offset<D, KIND>(tau, first + 1)) = f.z;
 }
 
 template <int D, int KIND>
-__device__ __forceinline__ void store_key(char* tile, int tau, int d0, h8_t x) {
-    RowFactors f = {};
-    if constexpr (KIND != KMI_KV_F16) f = row_factors<D / 8, KIND>(x);
-    const Packed<KIND> w = pack_row<KIND>(x, f);
+__device__ __forceinline__ void store_key(char* tile, int tau, int d0, const Packed<KIND>& w) {
     char* at = tile + kv_key_offset<D, KIND>(tau, d0);
     if constexpr (KIND == KMI_KV_F16) *reinterpret_cast<u4_t*>(at) = u4_t{w.w[0], w.w[1], w.w[2], w.w[3]};
     else if constexpr (KIND == KMI_KV_INT8) *reinterpret_cast<u2_t*>(at) = u2_t{w.w[0], w.w[1]};
     else *reinterpret_cast<uint32_t*>(at) = nibbles_apart(w.w[0]);
-    store_factors<D, KIND>(tile, tau, d0, 0, f);
 }
 
 // One token's value: its words stand 16 bytes apart.
@@ -132,70 +174,95 @@ __device__ __forceinline__ void store_value(char* tile, int tau, int d0, const P
     for (int i = 0; i < 8 / n; ++i)
         *reinterpret_cast<uint16_t*>(tile + kv_value_offset<D, KIND>(tau, d0 + n * i)) = (uint16_t)(w.w[i / 2] >> (16 * (i & 1)));
 }
-// Eight tokens tau0 .. tau0 + 7 (tau0 % 8 == 0): whole 16-byte chunks, 128 / n bytes in a row.
+// Eight tokens tau0 .. tau0 + 7 (tau0 % 8 == 0): whole 16-byte chunks, 128 / n bytes in a row; d0s: the quad's lanes' d0.
+// f16 and int8: four chunks of a quad at a time change hands, so that a store writes 64 bytes in a row instead of 16.
 template <int D, int KIND>
-__device__ __forceinline__ void store_values8(char* tile, int tau0, int d0, const Packed<KIND> (&w)[8]) {
-    constexpr int n = kv_per_word(KIND);
-    u4_t* at = reinterpret_cast<u4_t*>(tile + kv_value_offset<D, KIND>(tau0, d0));
+__device__ __forceinline__ void store_values8(char* tile, int tau0, const int (&d0s)[4], int lane, const Packed<KIND> (&w)[8]) {
+    constexpr int n = kv_per_word(KIND), CHUNKS = 8 / n;
+    u4_t c[CHUNKS];
 #pragma unroll
-    for (int i = 0; i < 8 / n; ++i) {
-        u4_t c;
+    for (int i = 0; i < CHUNKS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_perm(w[2 * j + 1].w[i / 2], w[2 * j].w[i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-        at[i] = c;
+        for (int j = 0; j < 4; ++j) c[i][j] = __builtin_amdgcn_perm(w[2 * j + 1].w[i / 2], w[2 * j].w[i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+    if constexpr (CHUNKS >= 4) {
+#pragma unroll
+        for (int q = 0; q < CHUNKS / 4; ++q) {
+            u4_t x[4] = {c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+            turn_quad(x, lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) reinterpret_cast<u4_t*>(tile + kv_value_offset<D, KIND>(tau0, d0s[k]))[4 * q + (lane & 3)] = x[k];
+        }
+    } else {
+        const int d0 = lane & 2 ? (lane & 1 ? d0s[3] : d0s[2]) : (lane & 1 ? d0s[1] : d0s[0]);
+        u4_t* at = reinterpret_cast<u4_t*>(tile + kv_value_offset<D, KIND>(tau0, d0));
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) at[i] = c[i];
+    }
+}
+// The same of keys: tokens tau0 + 4 h .. + 3 of a unit lie behind each other, 16 bytes apart, so four units of a quad change hands.
+template <int D, int KIND>
+__device__ __forceinline__ void store_keys8(char* tile, int tau0, const int (&d0s)[4], int lane, const Packed<KIND> (&w)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Packed<KIND> x[4] = {w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+        turn_quad(x, lane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_key<D, KIND>(tile, tau0 + 4 * h + (lane & 3), d0s[k], x[k]);
     }
 }
 
-// Cosines and sines of the pairs that a lane's eight elements d0 .. d0 + 7 belong to; NaN beyond the table.
+// A lane has two chunks of eight elements of a row, at da and db.  Half layout: in the turned part da and db = da + R/2 are
+// partners, element by element; interleaved: they are neighbours.  Behind the turned part they are neighbours.
 template <bool INTERLEAVED>
-struct Angles {
-    static constexpr int PAIRS = INTERLEAVED ? 4 : 8;
-    float c[PAIRS], s[PAIRS];
-    __device__ __forceinline__ void load(const float* table, int rows, int R, int pos, int d0) {
-        if (d0 >= R) return;
-        const bool inside = pos >= 0 && pos < rows;
-        const int i0 = INTERLEAVED ? d0 / 2 : d0 % (R / 2);
-        const f4_t* p = reinterpret_cast<const f4_t*>(table + (size_t)(inside ? pos : 0) * R + 2 * i0);
-#pragma unroll
-        for (int i = 0; i < PAIRS / 2; ++i) {
-            const f4_t v = p[i];
-            const float nan = __builtin_nanf("");
-            c[2 * i] = inside ? v[0] : nan; s[2 * i] = inside ? v[1] : nan;
-            c[2 * i + 1] = inside ? v[2] : nan; s[2 * i + 1] = inside ? v[3] : nan;
-        }
-    }
-    // x: the lane's elements; o: their partners (half layout)
-    __device__ __forceinline__ h8_t turn(h8_t x, h8_t o, int R, int d0) const {
-#pragma clang fp contract(off)
-        if (d0 >= R) return x;
-        h8_t y;
-        if constexpr (INTERLEAVED) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = (float)x[2 * i], b = (float)x[2 * i + 1];
-                y[2 * i] = (half_t)(a * c[i] - b * s[i]);
-                y[2 * i + 1] = (half_t)(b * c[i] + a * s[i]);
-            }
-        } else {
-            const bool first = d0 < R / 2;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float a = (float)x[e], b = (float)o[e];
-                const float t = b * s[e];
-                y[e] = (half_t)(a * c[e] + (first ? -t : t));
-            }
-        }
-        return y;
+struct Chunks {
+    int da, db;
+    bool turned;
+    int pair0;                                                  // first of the lane's eight pairs
+    __device__ __forceinline__ Chunks(int c, int R) {
+        turned = 16 * c < R;
+        da = !INTERLEAVED && turned ? 8 * c : 16 * c;
+        db = !INTERLEAVED && turned ? 8 * c + R / 2 : 16 * c + 8;
+        pair0 = 8 * c;
     }
 };
 
-// One workgroup: eight neighbouring positions 8 i .. 8 i + 7 of one sequence, 2048 / D rows (heads of queries, keys or values) of each;
-// a lane has eight elements of one row.  Where all eight tokens are there, all loads are in flight before the first use,
-// and the values leave as whole chunks of the cache, turned over in registers.
+// Turns a lane's two chunks by the angles of a position (NaN beyond the table).
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn(h8_t& a, h8_t& b, const float* table, int rows, int R, int pos, const Chunks<INTERLEAVED>& at) {
+#pragma clang fp contract(off)
+    if (!at.turned) return;
+    const bool inside = pos >= 0 && pos < rows;
+    const f4_t* p = reinterpret_cast<const f4_t*>(table + (size_t)(inside ? pos : 0) * R + 2 * at.pair0);
+    f4_t cs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = p[i];
+    if (!inside) {
+        const float nan = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = f4_t{nan, nan, nan, nan};
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float c = cs[i / 2][2 * (i & 1)], s = cs[i / 2][2 * (i & 1) + 1];
+        const float x = INTERLEAVED ? (float)(i < 4 ? a[2 * i & 7] : b[2 * i & 7]) : (float)a[i];
+        const float y = INTERLEAVED ? (float)(i < 4 ? a[(2 * i + 1) & 7] : b[(2 * i + 1) & 7]) : (float)b[i];
+        const half_t u = (half_t)(x * c - y * s), v = (half_t)(y * c + x * s);
+        if constexpr (INTERLEAVED) {
+            if (i < 4) { a[2 * i & 7] = u; a[(2 * i + 1) & 7] = v; }
+            else { b[2 * i & 7] = u; b[(2 * i + 1) & 7] = v; }
+        } else {
+            a[i] = u; b[i] = v;
+        }
+    }
+}
+
+// One workgroup: eight neighbouring positions 8 i .. 8 i + 7 of one sequence, 4096 / D rows (heads of queries, keys or values) of each;
+// a lane has sixteen elements of one row, both halves of its pairs.  Where all eight tokens are there, all loads are in flight
+// before the first use, and the values leave as whole chunks of the cache, turned over in registers.
 template <int D, int KIND, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
-    constexpr int LPR = D / 8, ROWS = 256 / LPR, K_ = KIND < 0 ? 0 : KIND;
-    const int b = blockIdx.y, d0 = (threadIdx.x % LPR) * 8, R = p.rotary_dim;
+    constexpr int LPR = D / 16, ROWS = 256 / LPR, K_ = KIND < 0 ? 0 : KIND;
+    const int b = blockIdx.y, R = p.rotary_dim, c = threadIdx.x % LPR;
     const int r = (p.q ? 0 : p.H) + blockIdx.z * ROWS + threadIdx.x / LPR;
     if (r >= p.H + p.KV + (KIND >= 0 ? p.KV : 0)) return;
     const bool is_q = r < p.H, is_v = r >= p.H + p.KV;
@@ -204,54 +271,66 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
     const int pos0 = (int)((unsigned)((start >> 3) + (int)blockIdx.x) << 3), s0 = (int)((unsigned)pos0 - (unsigned)start);
     if (s0 >= p.S) return;
 
+    const Chunks<INTERLEAVED> at(c, R);
+    int das[4], dbs[4];                                         // of the quad's lanes
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const Chunks<INTERLEAVED> o((c & ~3) + k, R);
+        das[k] = o.da; dbs[k] = o.db;
+    }
     const int heads = is_q ? p.H : p.KV;
     const half_t* row = is_q ? static_cast<const half_t*>(p.q) + b * p.q_batch : is_v ? static_cast<const half_t*>(p.v) + b * p.v_batch
                                                                                      : static_cast<const half_t*>(p.k) + b * p.k_batch;
     const int64_t step = is_q ? p.q_token : is_v ? p.v_token : p.k_token;
     row += (size_t)head * D;
     half_t* out = static_cast<half_t*>(is_q ? p.q_out : is_v ? nullptr : p.k_out);
-    if (out) out += ((size_t)b * p.S * heads + head) * D + d0;
+    if (out) out += ((size_t)b * p.S * heads + head) * D;
     const size_t out_step = (size_t)heads * D;
     const KvPlace place = {static_cast<char*>(p.cache), p.page_table, p.num_pages, p.page_tiles, p.max_pages, p.KV};
     char* tile = nullptr;                                       // the eight positions lie in one tile
     if constexpr (KIND >= 0) tile = is_q || pos0 < 0 ? nullptr : kv_tile_at<kv_tile_bytes(D, K_)>(place, b, head, pos0 / KV_TILE);
     const int tau0 = pos0 & (KV_TILE - 1);
-    const int partner = INTERLEAVED || d0 >= R ? d0 : d0 < R / 2 ? d0 + R / 2 : d0 - R / 2;
     const float* table = static_cast<const float*>(p.table);
-    Angles<INTERLEAVED> ang;
+    auto load = [&](int s, int d) { return *reinterpret_cast<const h8_t*>(row + s * step + d); };
+    auto store = [&](int s, int d, h8_t x) { *reinterpret_cast<h8_t*>(out + s * out_step + d) = x; };
 
     if (s0 >= 0 && s0 + 8 <= count) {
-        h8_t x[8];
+        h8_t xa[8], xb[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const h8_t*>(row + (s0 + j) * step + d0);
+        for (int j = 0; j < 8; ++j) { xa[j] = load(s0 + j, at.da); xb[j] = load(s0 + j, at.db); }
         if (is_v) {
             if constexpr (KIND >= 0) {
                 if (!tile) return;
-                Packed<K_> w[8];
+                Packed<K_> wa[8], wb[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    RowFactors f = {};
-                    if constexpr (K_ != KMI_KV_F16) f = row_factors<LPR, K_>(x[j]);
-                    w[j] = pack_row<K_>(x[j], f);
-                    store_factors<D, K_>(tile, tau0 + j, d0, kv_factors(K_) / 2, f);
+                    const RowFactors f = row_factors<LPR, K_>(xa[j], xb[j]);
+                    wa[j] = pack_row<K_>(xa[j], f);
+                    wb[j] = pack_row<K_>(xb[j], f);
+                    if (c == 0) store_factors<D, K_>(tile, tau0 + j, kv_factors(K_) / 2, f);
                 }
-                store_values8<D, K_>(tile, tau0, d0, w);
+                store_values8<D, K_>(tile, tau0, das, c, wa);
+                store_values8<D, K_>(tile, tau0, dbs, c, wb);
             }
             return;
         }
-        h8_t o[8];
-        if constexpr (!INTERLEAVED) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = *reinterpret_cast<const h8_t*>(row + (s0 + j) * step + partner);
-        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            ang.load(table, p.table_rows, R, pos0 + j, d0);
-            const h8_t y = ang.turn(x[j], INTERLEAVED ? x[j] : o[j], R, d0);
-            if (out) *reinterpret_cast<h8_t*>(out + (s0 + j) * out_step) = y;
-            if constexpr (KIND >= 0) {
-                if (tile) store_key<D, K_>(tile, tau0 + j, d0, y);
+            turn(xa[j], xb[j], table, p.table_rows, R, pos0 + j, at);
+            if (out) { store(s0 + j, at.da, xa[j]); store(s0 + j, at.db, xb[j]); }
+        }
+        if constexpr (KIND >= 0) {
+            if (!tile) return;
+            Packed<K_> wa[8], wb[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const RowFactors f = row_factors<LPR, K_>(xa[j], xb[j]);
+                wa[j] = pack_row<K_>(xa[j], f);
+                wb[j] = pack_row<K_>(xb[j], f);
+                if (c == 0) store_factors<D, K_>(tile, tau0 + j, 0, f);
             }
+            store_keys8<D, K_>(tile, tau0, das, c, wa);
+            store_keys8<D, K_>(tile, tau0, dbs, c, wb);
         }
         return;
     }
@@ -259,26 +338,24 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
         const int s = s0 + j;
         if (s < 0 || s >= p.S) continue;
         if (s >= count) {                                       // rows behind the sequence: zeros out, nothing into the cache
-            if (out) *reinterpret_cast<h8_t*>(out + s * out_step) = h8_t{};
+            if (out) { store(s, at.da, h8_t{}); store(s, at.db, h8_t{}); }
             continue;
         }
-        h8_t x = *reinterpret_cast<const h8_t*>(row + s * step + d0);
-        if (!is_v) {
-            const h8_t o = *reinterpret_cast<const h8_t*>(row + s * step + partner);
-            ang.load(table, p.table_rows, R, pos0 + j, d0);
-            x = ang.turn(x, o, R, d0);
-        }
-        if (out) *reinterpret_cast<h8_t*>(out + s * out_step) = x;
+        h8_t xa = load(s, at.da), xb = load(s, at.db);
+        if (!is_v) turn(xa, xb, table, p.table_rows, R, pos0 + j, at);
+        if (out) { store(s, at.da, xa); store(s, at.db, xb); }
         if constexpr (KIND >= 0) {
             if (!tile) continue;
+            const RowFactors f = row_factors<LPR, K_>(xa, xb);
+            const Packed<K_> wa = pack_row<K_>(xa, f), wb = pack_row<K_>(xb, f);
             if (is_v) {
-                RowFactors f = {};
-                if constexpr (K_ != KMI_KV_F16) f = row_factors<LPR, K_>(x);
-                store_value<D, K_>(tile, tau0 + j, d0, pack_row<K_>(x, f));
-                store_factors<D, K_>(tile, tau0 + j, d0, kv_factors(K_) / 2, f);
+                store_value<D, K_>(tile, tau0 + j, at.da, wa);
+                store_value<D, K_>(tile, tau0 + j, at.db, wb);
             } else {
-                store_key<D, K_>(tile, tau0 + j, d0, x);
+                store_key<D, K_>(tile, tau0 + j, at.da, wa);
+                store_key<D, K_>(tile, tau0 + j, at.db, wb);
             }
+            if (c == 0) store_factors<D, K_>(tile, tau0 + j, is_v ? kv_factors(K_) / 2 : 0, f);
         }
     }
 }
@@ -417,7 +494,7 @@ extern "C" int kmi_rope_kv(const kmi_rope_kv_args* args, void* stream) {
         if (rc < 0) return rc;
     }
     if (p.B == 0 || p.S == 0) return KMI_OK;
-    const int rows = (p.q ? p.H : 0) + p.KV + (cached ? p.KV : 0), at_once = 2048 / p.D;
+    const int rows = (p.q ? p.H : 0) + p.KV + (cached ? p.KV : 0), at_once = 4096 / p.D;
     const dim3 grid((unsigned)(((long long)p.S + 14) / 8), p.B, (rows + at_once - 1) / at_once), block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int kind = cached ? p.kind : -1;
