@@ -3,6 +3,7 @@
     python -m kairos_amd.bench_extra gemv70b   # decode-regime W4A16 on Llama-3-70B shapes, M = 1..32
     python -m kairos_amd.bench_extra convert   # int4 -> int8 / fp16 / tiled conversion on Qwen2.5-7B shapes
     python -m kairos_amd.bench_extra decoder   # random-init Llama-3-8B decoder: TTFT / TPOT / lane switches
+                                               # (--kv-cache f16|int8|int4: the library's paged cache, rotary positions and attention)
     python -m kairos_amd.bench_extra blasref   # the library's int8 / fp16 GEMMs of this image (hipBLASLt via torch) beside this build's
     python -m kairos_amd.bench_extra weightprep  # offline fp16 -> resident int4 format (device kernel vs host chain), W4A8 re-pack
     python -m kairos_amd.bench_extra actnorm   # per-token quantiser and fused residual add + RMSNorm + quantiser, GB/s
@@ -25,11 +26,14 @@ import torch
 from . import ops
 from .act_matching import MatchedRMSNorm, MatchedSiluMul
 from .dynamic_linear_v2 import COMP_TYPE_NAME, DynamicLinear     # version 2: the same classes plus the W4A8 lane
+from .kv_cache import PagedKVCache
 from .perf_profiler_v2 import Profiler
+from .rotary import rotary_table
 from .temp_cache import TempCache
 
 HBM = 8.0e12
 G = 128
+PAGE = 64                                                             # tokens a page of the decoder's cache
 
 
 def _weights(N, K, seed=10):
@@ -497,9 +501,11 @@ class _Layer(torch.nn.Module):
     """Pre-norm decoder layer over a static KV cache [B, kv_heads, T_max, d]: prefill fills positions 0..S-1, a
     decode step writes position `pos` (a device tensor, so the step is capturable) and attends under a mask.
     The residual stream travels as (x, delta) with hidden = x + delta: with `matched` norms the add, the norm and
-    the activation format of the consuming linear's lane come from one kernel (kairos_amd/act_matching.py)."""
+    the activation format of the consuming linear's lane come from one kernel (kairos_amd/act_matching.py).
+    kv_cache: None = that static cache and PyTorch glue; 'f16', 'int8' or 'int4' = the library's rotary positions, paged cache and
+    decode attention (kairos_amd/kv_cache.py).  A prefill attends to the values that the cache holds, as the steps after it do."""
 
-    def __init__(self, lin, dev, hidden=4096, heads=32, kv_heads=8, matched=True):
+    def __init__(self, lin, dev, hidden=4096, heads=32, kv_heads=8, matched=True, kv_cache=None):
         super().__init__()
         self.h, self.kv, self.d = heads, kv_heads, hidden // heads
         self.qkv, self.o, self.gate_up, self.down = lin
@@ -509,9 +515,13 @@ class _Layer(torch.nn.Module):
             self.n2 = MatchedRMSNorm(self.n2.weight, 1e-5, [self.gate_up])
             self.act = MatchedSiluMul([self.down])
         self.matched = matched
-        self.k_cache = self.v_cache = None
+        self.kv_cache = kv_cache
+        self.k_cache = self.v_cache = self.cache = None
 
     def alloc_cache(self, B, t_max, dev):
+        if self.kv_cache is not None:
+            self.cache = PagedKVCache(B * -(-t_max // PAGE), self.kv, self.d, self.kv_cache, PAGE, dev)
+            return
         self.k_cache = torch.zeros((B, self.kv, t_max, self.d), dtype=torch.float16, device=dev)
         self.v_cache = torch.zeros_like(self.k_cache)
 
@@ -523,10 +533,22 @@ class _Layer(torch.nn.Module):
         h = x if delta is None else x + delta
         return norm(h), h
 
-    def _qkv(self, x, delta, cs):
+    def _heads(self, x, delta):
+        """-> (hidden, output of the qkv linear [B, S, heads + 2 kv_heads, D])"""
         B, S, _ = x.shape
         y, x = self._norm(self.n1, x, delta)
-        qkv = self.qkv(y).view(B, S, self.h + 2 * self.kv, self.d)
+        return x, self.qkv(y).view(B, S, self.h + 2 * self.kv, self.d)
+
+    def _append(self, x, delta, paged, want_k=False):
+        """Turned queries (and keys), with this call's tokens in the paged cache; paged = (page table, positions int32 [B], rotary
+        table)."""
+        x, qkv = self._heads(x, delta)
+        pages, pos, table = paged
+        q, k, v = qkv.split((self.h, self.kv, self.kv), dim=2)
+        return x, self.cache.append(pages, pos, k, v, table, q=q, want_k=want_k), v
+
+    def _qkv(self, x, delta, cs):
+        x, qkv = self._heads(x, delta)
         qk = _rope(qkv[:, :, : self.h + self.kv], cs)                      # queries and keys rotated in one pass
         return (x, qk[:, :, : self.h].transpose(1, 2), qk[:, :, self.h:].transpose(1, 2),
                 qkv[:, :, self.h + self.kv:].transpose(1, 2))
@@ -540,13 +562,24 @@ class _Layer(torch.nn.Module):
         g, u = gu.chunk(2, dim=-1)
         return x, self.down(torch.nn.functional.silu(g) * u)
 
-    def prefill(self, x, delta):
+    def prefill(self, x, delta, paged=None):
         S = x.shape[1]
+        if paged is not None:
+            x, (q, k), v = self._append(x, delta, paged, want_k=True)
+            if self.kv_cache != "f16":                          # what was stored, not what was given
+                k, v = self.cache.read(paged[0], paged[1], S)
+            a = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
+                                                                 is_causal=S > 1, enable_gqa=True)
+            return self._mlp(x, a)
         x, q, k, v = self._qkv(x, delta, _rope_table(torch.arange(S, device=x.device), self.d, x.device))
         self.k_cache[:, :, :S] = k
         self.v_cache[:, :, :S] = v
         a = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=S > 1, enable_gqa=True)
         return self._mlp(x, a)
+
+    def paged_step(self, x, delta, paged, lens):
+        x, q, _ = self._append(x, delta, paged)
+        return self._mlp(x, self.cache.attend(q, paged[0], lens).transpose(1, 2))
 
     def step(self, x, delta, pos, mask, cs):
         """x, delta [B, 1, hidden]; pos int64 [1] on the device; mask bool [1, 1, 1, T_max], true up to pos; cs = rope
@@ -568,10 +601,12 @@ class Decoder:
     projection, greedy pick.  `linears[l]` = (qkv, o, gate_up, down) callables of layer l.  The decode step has fixed
     shapes (static KV cache, device-side position), so `capture()` records it into one HIP graph."""
 
-    def __init__(self, linears, dev, hidden=4096, heads=32, kv_heads=8, vocab=128256, matched=True, t_max=2048, seed=0):
-        self.dev, self.hidden, self.vocab, self.t_max = dev, hidden, vocab, t_max
+    def __init__(self, linears, dev, hidden=4096, heads=32, kv_heads=8, vocab=128256, matched=True, t_max=2048, seed=0,
+                 kv_cache=None):
+        self.dev, self.hidden, self.vocab, self.t_max, self.kv_cache = dev, hidden, vocab, t_max, kv_cache
         self.head_dim = hidden // heads
-        self.layers = [_Layer(lin, dev, hidden, heads, kv_heads, matched=matched) for lin in linears]
+        self.layers = [_Layer(lin, dev, hidden, heads, kv_heads, matched=matched, kv_cache=kv_cache) for lin in linears]
+        self.table = None if kv_cache is None else rotary_table(t_max, self.head_dim, 500000.0, device=dev)
         g = torch.Generator(device=dev).manual_seed(seed)
         self.emb = torch.randn(vocab, hidden, generator=g, device=dev, dtype=torch.float16) * 0.02
         self.head = torch.randn(vocab, hidden, generator=g, device=dev, dtype=torch.float16) * 0.02
@@ -586,19 +621,25 @@ class Decoder:
         self.pos = torch.zeros((1,), dtype=torch.int64, device=self.dev)
         self.tok = torch.zeros((B, 1), dtype=torch.int64, device=self.dev)
         self.logits = torch.zeros((B, 1, self.vocab), dtype=torch.float16, device=self.dev)
+        if self.kv_cache is not None:                                                        # one page table for all layers
+            per = -(-self.t_max // PAGE)
+            self.pages = torch.arange(B * per, dtype=torch.int32, device=self.dev).view(B, per)
+            self.zeros = torch.zeros((B,), dtype=torch.int32, device=self.dev)
+            self.pos_b = torch.zeros((B,), dtype=torch.int32, device=self.dev)
         self.graph = None
 
     def free(self):
         self.graph = None
         for L in self.layers:
-            L.k_cache = L.v_cache = None
+            L.k_cache = L.v_cache = L.cache = None
         torch.cuda.empty_cache()
 
     @torch.no_grad()
     def prefill_logits(self, ids):
         h, delta = self.emb[ids], None
+        paged = None if self.kv_cache is None else (self.pages, self.zeros, self.table)
         for L in self.layers:
-            h, delta = L.prefill(h, delta)
+            h, delta = L.prefill(h, delta, paged)
         return self.fnorm(h[:, -1:, :] + delta[:, -1:, :]) @ self.head.T                     # [B, 1, vocab]
 
     def prefill(self, ids):
@@ -606,11 +647,17 @@ class Decoder:
 
     @torch.no_grad()
     def step(self):
-        mask = (self.ar <= self.pos).view(1, 1, 1, self.t_max)
-        cs = _rope_table(self.pos, self.head_dim, self.dev)
         h, delta = self.x_in, None
-        for L in self.layers:
-            h, delta = L.step(h, delta, self.pos, mask, cs)
+        if self.kv_cache is None:
+            mask = (self.ar <= self.pos).view(1, 1, 1, self.t_max)
+            cs = _rope_table(self.pos, self.head_dim, self.dev)
+            for L in self.layers:
+                h, delta = L.step(h, delta, self.pos, mask, cs)
+        else:
+            lens, paged = self.pos_b + 1, (self.pages, self.pos_b, self.table)
+            for L in self.layers:
+                h, delta = L.paged_step(h, delta, paged, lens)
+            self.pos_b.add_(1)
         self.logits.copy_(self.fnorm(h + delta) @ self.head.T)
         nxt = self.logits.argmax(-1)
         self.tok.copy_(nxt)
@@ -620,6 +667,8 @@ class Decoder:
     def start(self, first, prompt_len):
         self.x_in.copy_(self.emb[first])
         self.pos.fill_(prompt_len)
+        if self.kv_cache is not None:
+            self.pos_b.fill_(prompt_len)
 
     def capture(self):
         """One warm-up step on a side stream, then the step recorded on that stream (the temp cache exists by then).
@@ -652,7 +701,7 @@ def decoder(args):
     nl = args.layers
     per_shape = [_layer(N, K, nl, dev) for N, K in shapes]
     dec = Decoder([[per_shape[s][l] for s in range(4)] for l in range(nl)], dev, matched=not args.torch_norm,
-                  t_max=args.prompt + args.new_tokens + 8)
+                  t_max=args.prompt + args.new_tokens + 8, kv_cache=None if args.kv_cache == "torch" else args.kv_cache)
     layers, vocab = dec.layers, dec.vocab
     names = {v: k for k, v in COMP_TYPE_NAME.items()}
 
@@ -728,7 +777,10 @@ def decoder(args):
         del graph
         dec.free()
     return {"bench": "decoder", "layers": nl, "prompt": args.prompt, "new_tokens": args.new_tokens,
-            "note": "random-init weights (one prepared layer cloned), fp16 SDPA attention in PyTorch over a static KV cache, "
+            "kv_cache": args.kv_cache,
+            "note": "random-init weights (one prepared layer cloned), "
+                    + ("fp16 SDPA attention in PyTorch over a static KV cache, " if args.kv_cache == "torch" else
+                       f"paged {args.kv_cache} KV cache with the library's rotary positions and decode attention (prefill attention: SDPA), ")
                     + ("norms and SiLU * up in PyTorch" if args.torch_norm else "residual add + RMSNorm, and SiLU * up, each with the "
                        "activation format of the next lane in one kernel (kmi_rmsnorm_quant_act, kmi_silu_mul_quant_act)") + ", greedy decoding",
             "norms": "torch" if args.torch_norm else "matched",
@@ -755,6 +807,8 @@ def main(argv=None):
     d.add_argument("--batches", type=int, nargs="+", default=[2, 4, 8, 16, 32])
     d.add_argument("--eager-decode", action="store_true", help="step token by token from Python instead of replaying a HIP graph")
     d.add_argument("--torch-norm", action="store_true", help="PyTorch residual adds, RMSNorms and SiLU * up instead of the fused matched operators")
+    d.add_argument("--kv-cache", choices=("torch", "f16", "int8", "int4"), default="torch", help="torch: static fp16 cache and PyTorch glue; "
+                   "else the library's paged cache of that kind, rotary positions and decode attention")
     d.add_argument("--check-tokens", type=int, default=8, help="tokens generated both eagerly and by replay, compared")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():

@@ -266,8 +266,9 @@ def _need_rows(x, name, what, device):
 
 def _launch_on(device, name, M, N, K, fn, args):
     """The call on the current stream of the tensors' device, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        return _call(name, M, N, K, fn, args, _stream())
+    idx = torch.cuda.current_device()
+    if device.index == idx:
+        return _call(name, M, N, K, fn, args, _raw_stream(idx) if _raw_stream is not None else _stream())
     with torch.cuda.device(device):
         return _call(name, M, N, K, fn, args, _stream())
 
@@ -283,7 +284,7 @@ def _rope_kv(what, q, k, v, start, table, interleaved, count, cache, page_table,
         H = q.shape[2]
         if q.shape[:2] != k.shape[:2] or q.shape[3] != D or H == 0:
             raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head_dim")
-        q_out = torch.empty((B, S, H, D), dtype=torch.float16, device=dev)
+        q_out = q.new_empty((B, S, H, D))
     cp = kind = pages = tiles = pp = width = 0
     if cache is not None:
         cd, kind = _cache_form(cache, what)
@@ -315,7 +316,7 @@ def rotary(q, k, start, table, interleaved=False, count=None):
     stands at start[b] + s (int32 [B]); table fp32 [positions, R / 2, 2] of cosines and sines (kairos_amd.rotary.rotary_table),
     R <= D a multiple of 16: the first R elements of a head turn in pairs (i, i + R/2), or (2i, 2i+1) when interleaved, the others are
     copied.  A position outside the table gives NaN.  Tokens s >= count[b] (int32 [B]) are padding and come back as zeros."""
-    k_out = torch.empty(k.shape, dtype=torch.float16, device=k.device)
+    k_out = k.new_empty(k.shape)
     q_out = _rope_kv("rotary", q, k, None, start, table, interleaved, count, None, None, k_out)
     return q_out, k_out
 
@@ -328,7 +329,7 @@ def kv_append(cache, page_table, start, k, v, table=None, q=None, interleaved=Fa
     cache uint8 [pages, KV, page_size / 32, kv_tile_bytes(D, kind)]; page_table int32 [B, pages a sequence]; q, k, v, start, table,
     interleaved, count as in rotary().  Position t of sequence b goes to page page_table[b, t // page_size]; a token whose page is not one
     of the cache is dropped, as is padding (s >= count[b]).  Two tokens of a call must not share a place."""
-    k_out = torch.empty(k.shape, dtype=torch.float16, device=k.device) if want_k else None
+    k_out = k.new_empty(k.shape) if want_k else None
     q_out = _rope_kv("kv_append", q, k, v, start, table, interleaved, count, cache, page_table, k_out)
     return (q_out, k_out) if want_k else q_out
 
@@ -375,7 +376,7 @@ def paged_attention(q, cache, page_table, lens, scale=None, window=0):
         raise ValueError(f"paged_attention: q {tuple(q.shape)} does not fit a cache of {KV} heads of {D}")
     pp, width = _need_pages(page_table, B, "paged_attention", dev)
     lp = _need_index(lens, (B,), "lens", "paged_attention", dev)
-    out = torch.empty(q.shape, dtype=torch.float16, device=dev)
+    out = q.new_empty(q.shape)
     if B:
         if dev.index != torch.cuda.current_device():
             with torch.cuda.device(dev):

@@ -436,6 +436,93 @@ def test_streams_of_their_own(ops):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_decoder_command_s_stack(ops, kind):
+    """The decoder command's layer (fused qkv, matched norms, switched linears) on the paged cache against the same layer on its static
+    fp16 cache and PyTorch attention, given the keys and values that a cache of this kind holds: prefill and decode logits, and graph
+    replays against eager steps token for token.  Both layers' keys and values are the same bits (same linears, same inputs), so
+    what differs are the roundings of attention and behind it: fp16 weights, attention output, three linears' outputs and the
+    activations between them, under 40 times 2^-11 of the largest logit."""
+    from kairos.dynamic_linear import DynamicLinear
+    from kairos.perf_profiler import Profiler
+    from kairos_amd.bench_extra import Decoder
+    from oracle import kairos_oracle as O
+    dev_ = torch.device("cuda:0")
+    hidden, heads, kv, mlp, vocab = 1024, 8, 2, 2048, 2048
+    d = hidden // heads
+    shapes = [((heads + 2 * kv) * d, hidden), (hidden, hidden), (2 * mlp, hidden), (hidden, mlp)]
+    prof = Profiler(shapes)
+    for sh in shapes:
+        for r, name in [(16, "w4a16_gemv"), (1 << 20, "w4a16_gemm")]:
+            prof.record_best_comp(sh, r, name)
+    old, DynamicLinear.prof = DynamicLinear.prof, prof
+    try:
+        lins = []
+        for layer in range(1):
+            ql = []
+            for i, (N, K) in enumerate(shapes):
+                lin = torch.nn.Linear(K, N, bias=False, dtype=torch.float16)
+                with torch.no_grad():
+                    lin.weight.copy_(torch.from_numpy(O.synth_weights(N, K, seed=300 + 10 * layer + i) * np.float16(2.0)))
+                ql.append(DynamicLinear.from_module(lin.cuda(), "cuda"))
+            lins.append(ql)
+        B, prompt, t_max = 3, 45, 160
+        paged = Decoder(lins, dev_, hidden, heads, kv, vocab, t_max=t_max, seed=1, kv_cache=kind)
+        glue = Decoder(lins, dev_, hidden, heads, kv, vocab, t_max=t_max, seed=1)
+        ids = torch.randint(0, vocab, (B, prompt), device=dev_, generator=torch.Generator(device=dev_).manual_seed(2))
+        tol = 40 * 2.0 ** -11
+        table = table_of(t_max, d, 500000.0)[0]
+
+        def held_qkv(layer):
+            def qkv_of(x, delta, cs):
+                x, qkv = layer._heads(x, delta)
+                pos = np.arange(qkv.shape[1])[None] if qkv.shape[1] > 1 else glue.pos.cpu().numpy()[None]
+                pos = np.broadcast_to(pos, qkv.shape[:2])
+                q, k, v = (t.cpu().numpy() for t in qkv.split((heads, kv, kv), dim=2))
+                q, k = rotated(q, pos, table, False), rotated(k, pos, table, False)
+                if kind != "f16":
+                    k, v = (DO.to_f16(DO.values_of(*DO.quantise(t, kind), kind, np.float32)) for t in (k, v))
+                return (x,) + tuple(dev(t).transpose(1, 2) for t in (q, k, v))
+            return qkv_of
+
+
+        def rel(a, b):
+            return ((a.float() - b.float()).abs().max() / b.float().abs().max()).item()
+
+        for layer in glue.layers:
+            layer._qkv = held_qkv(layer)
+        for dec in (paged, glue):
+            dec.alloc(B)
+        got, want = paged.prefill_logits(ids), glue.prefill_logits(ids)
+        assert torch.isfinite(got).all() and rel(got, want) < tol, rel(got, want)
+        first = want.argmax(-1)
+        eager = []
+        for dec in (paged, glue):
+            dec.start(first, prompt)
+        for t in range(4):
+            paged.step()
+            glue.step()
+            assert rel(paged.logits, glue.logits) < tol, (t, rel(paged.logits, glue.logits))
+            eager.append((paged.tok.clone(), paged.logits.clone()))
+            nxt = glue.tok                                          # both continue with the glue's token
+            paged.x_in.copy_(paged.emb[nxt])
+        paged.prefill(ids)
+        graph = paged.capture()
+        paged.start(first, prompt)
+        paged.prefill(ids)                                          # eager work between capture and replay
+        glue.start(first, prompt)
+        for t in range(4):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(paged.tok, eager[t][0]) and torch.equal(paged.logits, eager[t][1]), t
+            glue.step()
+            paged.x_in.copy_(paged.emb[glue.tok])
+        paged.free()
+        assert all(L.cache is None for L in paged.layers)
+    finally:
+        DynamicLinear.prof = old
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------------------
 def test_refusals(ops):
     q = torch.zeros((2, 3, 4, 64), dtype=torch.float16, device="cuda")
