@@ -19,8 +19,9 @@ static constexpr int pa_waves(int kind) { return kind == KMI_KV_INT4 ? 8 : 4; }
 // Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (182 us against 191 for 2 x 131072 f16: fewer places of
 // memory at once), 512 hide the starts and ends of short tasks (19 sequences of up to 7985, int8, 64 wide: 20 us against 29).
 static constexpr int PA_LONG = 96;            // tiles a share from which 256 uneven ones are taken all the same
-// A share below six tiles a wave does not pay its join, which costs about 5 us (511 tokens of 8 heads, int4: 9.0 us whole, 11.4 cut).
-static constexpr int PA_MIN_STEPS = 6;
+// Being cut costs a task about 3 us (hand-off and join): none of up to nine tiles a wave is (2 x 1152 f16, 36 tiles: 9.6 us
+// whole, 10.6 cut), and no share is smaller than three (1 x 4096 f16: 11.8 us, 13.2 with six).
+static constexpr int PA_WHOLE_STEPS = 9, PA_MIN_STEPS = 3;
 static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start and end; 3 and 12 measured the same
 // Tiles of the page table from which a wave takes 32 query heads at once (more than 16 share a key head): the cache is read once
 // (64 x 62479 int8, 20 heads: 115 us against 176), but there are half as many shares (13 x up to 7411 int4: 21 us against 14).
@@ -265,34 +266,15 @@ struct PaWave {
             psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w, psum, 0, 0, 0);
         }
     }
-    // The sums as they stand: over the lane groups, and for codes the units, the codes' middle (taken off with the very
-    // weights that entered the products, so their rounding cancels) and the offsets.  PACK 2: the two halves joined, in both.
-    __device__ __forceinline__ void finish() {
-        l = group_sum(l);
-        if constexpr (CODES) {
-            if constexpr (KIND == KMI_KV_INT4) zsum = group_sum(zsum);
-            const float off = KIND == KMI_KV_INT8 ? 128.0f * psum[0] : 8.0f * psum[0];
-#pragma unroll
-            for (int T = 0; T < OT; ++T) {
-                const float unit = KIND == KMI_KV_INT4 && (T & 1) ? 0x1p20f : 0x1p24f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[T][r] = __builtin_fmaf(acc[T][r], unit, -off) + zsum;
-            }
-        }
-        if constexpr (PACK == 2) {
-            const float m2 = fmaxf(m, other_half(m)), a = __builtin_amdgcn_exp2f(m - m2);
-            m = m2;
-            l *= a;
-            l += other_half(l);
-#pragma unroll
-            for (int T = 0; T < OT; ++T)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = acc[T][r] * a;
-                    acc[T][r] = x + other_half(x);
-                }
-        }
+    // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output -- the offsets,
+    // less the codes' middle times the very weights that entered the products, so that their rounding cancels.
+    __device__ __forceinline__ void totals(float& sum, float& add) const {
+        sum = group_sum(l);
+        add = 0.0f;
+        if constexpr (KIND == KMI_KV_INT8) add = -128.0f * psum[0];
+        if constexpr (KIND == KMI_KV_INT4) add = group_sum(zsum) - 8.0f * psum[0];
     }
+    static __device__ __forceinline__ float unit_of(int T) { return !CODES ? 1.0f : KIND == KMI_KV_INT4 && (T & 1) ? 0x1p20f : 0x1p24f; }
     static __device__ __forceinline__ float other_half(float v) {          // row_ror 8: column c ^ 8 of the same lane group
         return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
     }
@@ -346,18 +328,103 @@ struct Flag {
     static constexpr bool value = V;
 };
 
-// Four waves' sums, each relative to its own reference: wave v adds up the output tiles T = v * D / 64 .. of all four.
-template <int D>
+// The waves' sums, each relative to its own reference.
+template <int D, int NW>
 struct PaJoin {
-    float m[4][16], l[4][16];
-    f4_t o[4][D / 16][64];
+    float m[NW][16], l[NW][16], add[NW][16];
+    f4_t o[NW][D / 16][64];
 };
+
+// Slot of share v of a task that begins in share w0.
+__device__ __forceinline__ size_t pa_slot(int w0, int v, int slot) { return ((size_t)(w0 + v) * 2 + (v == 0)) * slot; }
+
+// n shares' sums to the task's outputs, by all 64 NW threads: four outputs a thread and share, the shares dealt over the threads that
+// are left, their references and sums in LDS first.  One workgroup reads slowly past its caches (about 10 GB/s): all loads of a
+// thread are in flight at once.
+template <int D, int HT, int NW>
+__device__ __forceinline__ void join_shares(const float* partial, int slot, int w0, int n, int used, half_t* out, float* lds, int room) {
+    constexpr int COLS = 16 * HT, THREADS = 64 * NW, FLIGHT = 8;
+    const int quads = used * D / 4;                              // groups of four outputs
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(partial), 0, -1, 0x00020000);
+    const int most = room / 2 / (2 * COLS);                      // shares whose references fit half of the LDS at once
+    float* held = lds;                                           // [share][column] reference, sum
+    f4_t* outs = reinterpret_cast<f4_t*>(lds + room / 2);        // [dealt][quads] partial outputs
+    const int dealt = max(1, min(min(THREADS / quads, n), room / 2 / (4 * quads)));
+    for (int q0 = 0; q0 < quads; q0 += THREADS) {
+        const int q = dealt > 1 ? threadIdx.x % quads : q0 + threadIdx.x, first = dealt > 1 ? threadIdx.x / quads : 0;
+        const int c = min(4 * q / D, used - 1), at = c / 16 * (32 + 16 * D) + 32 + 4 * q - c / 16 * 16 * D;
+        const bool mine = q < quads && first < dealt;
+        float top = PA_NEG, sum = 0.0f;
+        f4_t o = {};
+        for (int v0 = 0; v0 < n; v0 += most) {
+            const int here = min(most, n - v0);
+            __syncthreads();
+            for (int i = threadIdx.x; i < here * COLS; i += THREADS) {
+                const int k = i % COLS;
+                if (k >= used) continue;
+                const float* s = partial + pa_slot(w0, v0 + i / COLS, slot) + k / 16 * (32 + 16 * D) + k % 16;
+                held[2 * i] = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                held[2 * i + 1] = __hip_atomic_load(s + 16, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (!mine) continue;
+            for (int v = first; v < here; v += FLIGHT * dealt) {
+                f4_t y[FLIGHT];
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k) {              // 16 = sc1: performed at the memory side, as the stores were
+                    const int share = v0 + min(v + k * dealt, here - 1);
+                    y[k] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)((pa_slot(w0, share, slot) + at) * 4), 0, 16));
+                }
+                float next = top, m[FLIGHT];
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k) {
+                    m[k] = v + k * dealt < here ? held[2 * ((v + k * dealt) * COLS + c)] : PA_NEG;
+                    next = fmaxf(next, m[k]);
+                }
+                const float keep = __builtin_amdgcn_exp2f(top - next);
+                sum *= keep; o = o * keep; top = next;
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k) {
+                    if (v + k * dealt >= here) continue;
+                    const float f = __builtin_amdgcn_exp2f(m[k] - next);
+                    sum += f * held[2 * ((v + k * dealt) * COLS + c) + 1];
+                    o = o + y[k] * f;
+                }
+            }
+        }
+        if (dealt > 1) {                                         // the threads that share an output, in order
+            float* tops = held;                                  // [dealt][quads] reference, sum
+            __syncthreads();
+            if (mine) {
+                outs[first * quads + q] = o;
+                tops[2 * (first * quads + q)] = top;
+                tops[2 * (first * quads + q) + 1] = sum;
+            }
+            __syncthreads();
+            if (mine && first == 0) {
+                for (int k = 1; k < dealt; ++k) {
+                    const float m = tops[2 * (k * quads + q)], next = fmaxf(top, m);
+                    const float keep = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+                    sum = sum * keep + f * tops[2 * (k * quads + q) + 1];
+                    o = o * keep + outs[k * quads + q] * f;
+                    top = next;
+                }
+            }
+        }
+        if (mine && first == 0) {
+            const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<h4*>(out + 4 * q) = h4{(half_t)(o[0] * norm), (half_t)(o[1] * norm), (half_t)(o[2] * norm), (half_t)(o[3] * norm)};
+        }
+        if (dealt > 1) break;
+    }
+}
 
 template <int D, int KIND, int PACK, int HT>
 __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 256 ? 1 : 2) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
-    constexpr int NW = pa_waves(KIND), MINE = D / 64;
+    constexpr int NW = pa_waves(KIND), MINE = D / 16 / NW > 0 ? D / 16 / NW : 1;         // MINE: output tiles that a wave joins
     using W = PaWave<D, KIND, PACK>;
-    __shared__ PaJoin<D> join;
+    __shared__ PaJoin<D, NW> join;
     __shared__ int last;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int G = p.H / p.KV, run = blockIdx.x;
@@ -376,7 +443,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
     // One workgroup a CU where the shares come out even or are long, else as many as there are.
     const int units = sum_over([](int n) { return n; }), most = gridDim.x;
     auto quota_of = [&](int units, int shares) { return (max((units + shares - 1) / shares, PA_MIN_STEPS * NW) + NW - 1) / NW * NW; };
-    auto pieces_of = [](int n, int q) { return n <= PA_MIN_STEPS * NW * 3 / 2 ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
+    auto pieces_of = [](int n, int q) { return n <= PA_WHOLE_STEPS * NW ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
     auto pieces = [&](int q) { return sum_over([&](int n) { return pieces_of(n, q); }); };
     int shares = min(most, 256), quota = quota_of(units, shares);
     bool even = pieces(quota) <= shares;
@@ -497,54 +564,45 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
         half_t* out = out0 + ((size_t)b * p.H + head * G + h0) * D;
 #pragma unroll
         for (int x = 0; x < HT; ++x) {
-            w[x].finish();
             if (x > 0) __syncthreads();                        // the arrays are written again
+            float sum, add;
+            w[x].totals(sum, add);
+            if (g == 0) { join.m[wave][col] = w[x].m; join.l[wave][col] = sum; join.add[wave][col] = add; }
 #pragma unroll
-            for (int f = NW / 4 - 1; f >= 0; --f) {            // four waves at a time: the second four hand over to the first
-                if (wave / 4 == f) {
-                    if (g == 0) { join.m[wave & 3][col] = w[x].m; join.l[wave & 3][col] = w[x].l; }
+            for (int T = 0; T < W::OT; ++T) join.o[wave][T][lane] = w[x].acc[T];
+            __syncthreads();
+            float mm = PA_NEG, ll = 0.0f, plus = 0.0f, a[NW];
 #pragma unroll
-                    for (int T = 0; T < W::OT; ++T) join.o[wave & 3][T][lane] = w[x].acc[T];
-                }
-                __syncthreads();
-                if (f > 0) {
-                    if (wave / 4 == f - 1) {
-                        const float m1 = join.m[wave & 3][col], m2 = fmaxf(w[x].m, m1);
-                        const float a0 = __builtin_amdgcn_exp2f(w[x].m - m2), a1 = __builtin_amdgcn_exp2f(m1 - m2);
-                        w[x].l = w[x].l * a0 + join.l[wave & 3][col] * a1;
-                        w[x].m = m2;
+            for (int v = 0; v < NW; ++v) mm = fmaxf(mm, join.m[v][col]);
+            if constexpr (PACK == 2) mm = fmaxf(mm, W::other_half(mm));
 #pragma unroll
-                        for (int T = 0; T < W::OT; ++T) w[x].acc[T] = w[x].acc[T] * a0 + join.o[wave & 3][T][lane] * a1;
-                    }
-                    __syncthreads();
-                }
-            }
-            float mm = PA_NEG, ll = 0.0f, a[4];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) mm = fmaxf(mm, join.m[v][col]);
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < NW; ++v) {
                 a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
                 ll += a[v] * join.l[v][col];
+                plus += a[v] * join.add[v][col];
             }
+            if constexpr (PACK == 2) { ll += W::other_half(ll); plus += W::other_half(plus); }
             const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
             float* part = slot + x * (32 + 16 * D);
-            if (wave < 4 && col + 16 * x < used) {
+            if (wave * MINE < W::OT) {
 #pragma unroll
                 for (int i = 0; i < MINE; ++i) {
                     const int T = wave * MINE + i;
                     f4_t o = {};
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) o = o + join.o[v][T][lane] * a[v];
+                    for (int v = 0; v < NW; ++v) o = o + join.o[v][T][lane] * a[v];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
+                        float y = o[r];
+                        if constexpr (PACK == 2) y += W::other_half(y);
+                        if constexpr (W::CODES) y = __builtin_fmaf(y, W::unit_of(T), plus);
+                        if ((PACK == 2 && col >= 8) || col + 16 * x >= used) continue;
                         const int d = W::d_of(T, 4 * g + r);
-                        const float y = o[r];
                         if (complete) out[(size_t)(col + 16 * x) * D + d] = (half_t)(y * norm);
                         else __hip_atomic_store(part + 32 + col * D + d, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     }
                 }
-                if (!complete && wave == 0 && g == 0) {
+                if (!complete && wave == 0 && g == 0 && col + 16 * x < used && !(PACK == 2 && col >= 8)) {
                     __hip_atomic_store(part + col, mm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     __hip_atomic_store(part + 16 + col, ll, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
@@ -559,24 +617,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
             if (threadIdx.x == 0) last = __hip_atomic_fetch_add(sp.counters + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(n - 1);
             __syncthreads();
             if (last) {
-                auto slot_of = [&](int v) { return sp.partial + ((size_t)(w0 + v) * 2 + (v == 0)) * sp.slot; };
-                for (int i = threadIdx.x; i < used * D; i += 64 * NW) {
-                    const int hc = i / D % 16, x = i / (16 * D);
-                    float top = PA_NEG, sum = 0.0f, o = 0.0f;
-#pragma unroll 4
-                    for (int v = 0; v < n; ++v) {
-                        const float* s = slot_of(v) + x * (32 + 16 * D);
-                        const float mv = __hip_atomic_load(s + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        const float lv = __hip_atomic_load(s + 16 + hc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        const float ov = __hip_atomic_load(s + 32 + i % (16 * D), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        const float next = fmaxf(top, mv);
-                        const float keep = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(mv - next);
-                        sum = sum * keep + f * lv;
-                        o = o * keep + f * ov;
-                        top = next;
-                    }
-                    out[i] = (half_t)(sum == 0.0f ? 0.0f : o / sum);
-                }
+                join_shares<D, HT, NW>(sp.partial, sp.slot, w0, n, used, out, reinterpret_cast<float*>(join.o), sizeof(join.o) / sizeof(float));
                 if (threadIdx.x == 0) __hip_atomic_store(sp.counters + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the next call
             }
         }
