@@ -462,9 +462,9 @@ int kv_check_cache(const char* fn, const void* cache, const void* page_table, in
     if (!kmi_aligned16(cache)) return kmi_set_error(KMI_E_ALIGN, "%s: the cache must be 16-byte aligned", fn);
     if (kmi_kv_tile_bytes(D, kind) < 0) return KMI_E_SHAPE;
     if (B < 0 || B > 65535 || KV <= 0 || num_pages <= 0 || page_tiles <= 0 || max_pages <= 0 ||
-        (long long)max_pages * page_tiles > (1ll << 26))
-        return kmi_set_error(KMI_E_SHAPE, "%s: need 0<=B<=65535, KV>0, num_pages>0, page_tiles>0, max_pages>0 and at most 2^31 tokens a "
-                             "sequence (B=%d KV=%d num_pages=%d page_tiles=%d max_pages=%d)", fn, B, KV, num_pages, page_tiles, max_pages);
+        (long long)max_pages * page_tiles >= (1ll << 26) || (double)num_pages * KV * page_tiles > 2147483647.0)
+        return kmi_set_error(KMI_E_SHAPE, "%s: need 0<=B<=65535, KV>0, num_pages>0, page_tiles>0, max_pages>0, under 2^31 tokens a sequence "
+                             "and under 2^31 tiles (B=%d KV=%d num_pages=%d page_tiles=%d max_pages=%d)", fn, B, KV, num_pages, page_tiles, max_pages);
     return KMI_OK;
 }
 

@@ -136,24 +136,45 @@ def get_tile(tile, D, kind):
     return out[0], out[1]
 
 
+_PLACES = {}
+
+
+def get_tiles(tiles, D, kind):
+    """Keys and values fp64 [n, 32, D] of tiles uint8 [n, tile_bytes]: get_tile by whole index arrays."""
+    if (D, kind) not in _PLACES:
+        _PLACES[D, kind] = [np.array([[place(tau, d, D, kind) for d in range(D)] for tau in range(TILE)]) for place in (key_place, value_place)]
+    out = []
+    for part, at in enumerate(_PLACES[D, kind]):
+        byte, shift = at[..., 0], at[..., 1]
+        if kind == "f16":
+            out.append(np.stack((tiles[:, byte], tiles[:, byte + 1]), -1).view(np.float16)[..., 0].astype(np.float64))
+            continue
+        u = (tiles[:, byte].astype(np.int64) >> shift) & (255 if kind == "int8" else 15)
+        per = FACTORS[kind] // 2
+
+        def factor(i):
+            lo = np.array([factor_place(tau, i, D, kind) for tau in range(TILE)])
+            return np.stack((tiles[:, lo], tiles[:, lo + 1]), -1).view(np.float16)[..., 0]
+
+        out.append(values_of(u, factor(per * part), factor(per * part + 1) if kind == "int4" else np.float16(0), kind))
+    return out
+
+
 def sequence(cache, page_row, length, head, D, kind):
     """Keys and values fp64 [length, D] of one head of one sequence."""
-    tiles_per_page = cache.shape[2]
-    ks, vs = [], []
-    for t in range(-(-length // TILE)):
-        k, v = get_tile(cache[page_row[t // tiles_per_page], head, t % tiles_per_page], D, kind)
-        ks.append(k)
-        vs.append(v)
-    if not ks:
+    if not length:
         return np.zeros((0, D)), np.zeros((0, D))
-    return np.concatenate(ks)[:length], np.concatenate(vs)[:length]
+    per = cache.shape[2]
+    t = np.arange(-(-length // TILE))
+    k, v = get_tiles(cache[np.asarray(page_row)[t // per], head, t % per], D, kind)
+    return k.reshape(-1, D)[:length], v.reshape(-1, D)[:length]
 
 
 def attend(q, k, v, scale):
-    """q fp16 [G, D], k, v fp64 [T, D] -> (o fp64 [G, D], sum p |v| / sum p, sum p) with p relative to the largest."""
+    """q fp16 [G, D], k, v fp64 [T, D] -> (o fp64 [G, D], sum p |v| / sum p, sum p with p relative to the largest, p / sum p)."""
     if not len(k):
-        return np.zeros(q.shape), np.zeros(q.shape), np.zeros((len(q), 1))
+        return np.zeros(q.shape), np.zeros(q.shape), np.zeros((len(q), 1)), np.zeros((len(q), 0))
     s = q.astype(np.float64) @ k.T * scale
     p = np.exp(s - s.max(-1, keepdims=True))
     t = p.sum(-1, keepdims=True)
-    return p @ v / t, p @ np.abs(v) / t, t
+    return p @ v / t, p @ np.abs(v) / t, t, p / t

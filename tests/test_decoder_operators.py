@@ -72,6 +72,7 @@ def test_oracle_token_round_trip():
         for tau in range(32):
             DO.put_token(tile, tau, k[tau], v[tau], kind)
         gk, gv = DO.get_tile(tile, 64, kind)
+        assert all(np.array_equal(a[0], b) for a, b in zip(DO.get_tiles(tile[None], 64, kind), (gk, gv)))
         for x, got in ((k, gk), (v, gv)):
             if kind == "f16":
                 assert np.array_equal(got, x.astype(np.float64))
@@ -148,7 +149,8 @@ def _pack(form, base, change):
     (dict(D=96), -2), (dict(D=0), -2), (dict(B=-1), -2), (dict(B=65536), -2), (dict(S=-1), -2), (dict(KV=0), -2), (dict(H=0), -2),
     (dict(H=70000), -2), (dict(rotary_dim=72), -2), (dict(rotary_dim=24), -2), (dict(rotary_dim=-16), -2), (dict(table=0), -2),
     (dict(table_rows=0), -2), (dict(kind=3), -2), (dict(kind=-1), -2), (dict(num_pages=0), -2), (dict(page_tiles=0), -2),
-    (dict(max_pages=0), -2), (dict(max_pages=1 << 20, page_tiles=1 << 10), -2), (dict(B=0), 0), (dict(S=0), 0),
+    (dict(max_pages=0), -2), (dict(max_pages=1 << 20, page_tiles=1 << 10), -2), (dict(max_pages=1 << 26), -2),
+    (dict(num_pages=1 << 28, KV=8), -2), (dict(B=0), 0), (dict(S=0), 0),
 ])
 def test_rope_kv_refusals(lib, change, code):
     from kairos_amd import ops

@@ -190,11 +190,14 @@ def test_rows_that_are_not_finite_read_as_nan(ops, kind):
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------------
-def attention_bound(q, k, v, scale, kind, o, mean_v, total):
+def attention_bound(q, k, v, scale, kind, o, mean_v, total, weights):
     """How far the kernel may be off: the output's rounding (2^-11), the weights' rounding to fp16 (2^-11 of each, half a subnormal
     step of the smallest), and the scores' error -- D products added in fp32, codes with their offset (at most 1152 + 127, or
     1024 + 15) in front of the subtraction -- which moves a weight by as much, relative.  The sums over tokens are fp32: T * 2^-24
-    of the mean size."""
+    of the mean size.
+    Codes: what is summed are the codes themselves, 0..255 or 0..15, not the values, and the offsets come off the sums: T + 8 additions
+    (the join and the subtraction among them), each off by 2^-24 of a sum of at most p times the row's width, 255 s = 2 max|v| for
+    int8 and 15 s + |z| + 8 s <= 4 max|v| for int4.  An element that is zero in the row with all the weight shows it: there mean_v is nothing."""
     T, D = k.shape
     if T == 0:
         return np.zeros(o.shape)
@@ -202,7 +205,9 @@ def attention_bound(q, k, v, scale, kind, o, mean_v, total):
     kmax = np.abs(k).max()
     big = {"f16": kmax, "int8": kmax / 100 * 1300, "int4": kmax * 1200}[kind]
     err = scale * aq * big * (D / 8 + 8) * 2.0 ** -24 + 2.0 ** -20
-    return (np.abs(o) + mean_v) * 2.0 ** -11 + 2 * mean_v * (err + T * 2.0 ** -24) + T * 2.0 ** -25 * np.abs(v).max() / total + 2.0 ** -24
+    width = 0.0 if kind == "f16" else (weights @ np.abs(v).max(-1))[:, None] * {"int8": 2, "int4": 4}[kind]
+    return ((np.abs(o) + mean_v) * 2.0 ** -11 + 2 * mean_v * (err + T * 2.0 ** -24) + T * 2.0 ** -25 * np.abs(v).max() / total + 2.0 ** -24
+            + (T + 8) * 2.0 ** -24 * width)
 
 
 def random_cache(rng, pool, KV, tiles, D, kind):
@@ -243,8 +248,8 @@ def check_attention(ops, cache, pages, lens, q, KV, D, kind, window=0, scale=Non
         for h in range(KV):
             k, v = DO.sequence(cache, pages[b], n, h, D, kind)
             k, v = k[lo:], v[lo:]
-            o, mean_v, total = DO.attend(q[b, h * G:(h + 1) * G], k, v, sc)
-            bound = attention_bound(q[b, h * G:(h + 1) * G], k, v, sc, kind, o, mean_v, total)
+            o, mean_v, total, weights = DO.attend(q[b, h * G:(h + 1) * G], k, v, sc)
+            bound = attention_bound(q[b, h * G:(h + 1) * G], k, v, sc, kind, o, mean_v, total, weights)
             off = np.abs(got[b, h * G:(h + 1) * G] - o)
             assert (off <= bound).all(), (b, h, n, float((off / np.maximum(bound, 1e-30)).max()))
 
@@ -338,6 +343,132 @@ def test_cache_beyond_32_bit_offsets(ops, kind):
     for a, b in zip(*outs):
         assert torch.isfinite(a).all() and torch.equal(a, b)
     del cache
+
+
+def appended(ops, rng, lens, KV, D, kind, page, width=None, size=1.0):
+    """A cache filled by kv_append (whose bytes the oracle has checked), its page table (-1 behind a sequence's pages) as numpy."""
+    need = [-(-n // page) for n in lens]
+    pool = sum(need) + 2
+    order, at = rng.permutation(pool), 0
+    pages = np.full((len(lens), width or max(max(need), 1)), -1, np.int32)
+    for b, n in enumerate(need):
+        pages[b, :n] = order[at:at + n]
+        at += n
+    cache = torch.full((pool, KV, page // 32, ops.kv_tile_bytes(D, kind)), 255, dtype=torch.uint8, device="cuda")      # NaN patterns
+    S = max(max(lens), 1)
+    k, v = (dev((rng.standard_normal((len(lens), S, KV, D)) * size).astype(np.float16)) for _ in range(2))
+    ops.kv_append(cache, dev(pages), torch.zeros(len(lens), dtype=torch.int32, device="cuda"), k, v, count=i32(*lens))
+    return cache, pages
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B, KV, lens", [
+    (130, 4, lambda i: (i * 37) % 41),                            # more tasks than shares, sequences of no tokens among them
+    (70, 8, lambda i: 1 + (i * 53) % 200),
+    (3, 2, lambda i: (5000, 1, 1700)[i]),                         # pieces of equal length
+    (40, 8, lambda i: 9000 if i == 7 else 1 + (i * 11) % 60),    # one long sequence among short ones: a row cut anywhere
+    (257, 1, lambda i: i),                                         # more than 64 lengths, tasks of every length up to 256
+])
+def test_attention_work_shared_out(ops, B, KV, lens, kind):
+    """Every way the tiles are shared out over workgroups: whole tasks, equal pieces, a row of tasks cut anywhere."""
+    D, H = 64, 4 * KV
+    lens = [lens(i) for i in range(B)]
+    rng = np.random.default_rng(B)
+    cache, pages = appended(ops, rng, lens, KV, D, kind, 32)
+    q = (rng.standard_normal((B, H, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    again = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))          # whichever workgroup joins
+    ws = ops.gemv_workspace_for("cuda")
+    assert not ws[:65536].any()                                                 # arrival counters left zero
+    some = sorted(set([0, B - 1, int(np.argmax(lens))] + list(rng.choice(B, min(B, 24), replace=False))))
+    check_attention(ops, cache.cpu().numpy(), pages[some], [lens[i] for i in some], q[some], KV, D, kind, got=got[some])
+    none = [i for i, n in enumerate(lens) if n == 0]
+    assert not got[none].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, G", [(64, 17), (64, 32), (64, 33), (128, 20), (128, 64), (256, 20)])
+def test_attention_many_heads_on_a_wide_page_table(ops, D, G, kind):
+    """Page tables with room for far longer sequences: 32 query heads at once where more than 16 share a key head, one sequence cut."""
+    lens = [2200, 70, 0]
+    rng = np.random.default_rng(G)
+    cache, pages = appended(ops, rng, lens, 1, D, kind, 32, width=5000)
+    q = (rng.standard_normal((3, G, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    check_attention(ops, cache.cpu().numpy(), pages, lens, q, 1, D, kind, got=got)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_flat_and_peaked_over_many_tokens(ops, kind):
+    """20000 equal scores (every token counts alike: sums of many small weights) and one token far above the others."""
+    D, n = 128, 20000
+    rng = np.random.default_rng(8)
+    cache, pages = appended(ops, rng, [n, n], 1, D, kind, 64)
+    q = np.zeros((2, 8, D), np.float16)
+    k, _ = DO.sequence(cache.cpu().numpy(), pages[1], n, 0, D, kind)
+    q[1] = (k[12345] * 3).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(n, n))
+    check_attention(ops, cache.cpu().numpy(), pages, [n, n], q, 1, D, kind, got=got)
+
+
+def test_attention_values_that_are_infinite_where_no_token_counts(ops):
+    """f16: infinities and NaN in keys and values in front of the window and behind the end."""
+    rng = np.random.default_rng(3)
+    D, n, w = 64, 75, 20
+    cache, pages = filled(rng, [n], 1, D, "f16", 32)
+    for t in (0, 31, 40, n - w - 1):
+        bad = np.full(D, np.inf if t % 2 else np.nan, np.float16)
+        DO.put_token(cache[pages[0, t // 32], 0, 0], t % 32, bad, bad, "f16")
+    q = rng.standard_normal((1, 4, D)).astype(np.float16)
+    check_attention(ops, cache, pages, [n], q, 1, D, "f16", window=w)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_graphs_of_cut_sequences_on_one_scratch(ops, kind):
+    """Captured calls whose sequences are cut into shares, two graphs in turn on the scratch that they share, eager calls in between."""
+    rng = np.random.default_rng(6)
+    D, H, KV = 128, 8, 2
+    lens = i32(4000, 2600)
+    cache, pages = appended(ops, rng, [4000, 2600], KV, D, kind, 64)
+    pd = dev(pages)
+    qs = [torch.randn((2, H, D), dtype=torch.float16, device="cuda") for _ in range(2)]
+    scratch, side = ops.Scratch(), torch.cuda.Stream()
+    graphs = []
+    side.wait_stream(torch.cuda.current_stream())
+    for q in qs:
+        with torch.cuda.stream(side), scratch:
+            ops.paged_attention(q, cache, pd, lens)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with scratch, torch.cuda.graph(g, stream=side):
+            out = ops.paged_attention(q, cache, pd, lens)
+        graphs.append((g, out))
+    for i in range(4):
+        for q in qs:
+            q.copy_(torch.randn(q.shape, dtype=torch.float16, device="cuda"))
+        for g, _ in graphs:
+            g.replay()
+        want = [ops.paged_attention(q, cache, pd, lens) for q in qs]
+        torch.cuda.synchronize()
+        for (_, out), w in zip(graphs, want):
+            assert torch.equal(out.view(torch.int16), w.view(torch.int16)), i
+        lens.sub_(i32(100, 700))
+    assert not scratch.gemv[:65536].any()
+
+
+def test_capture_without_a_scratch_is_refused(ops):
+    """As every call of the library that needs one: creating a scratch inside a capture would record a fill into the graph."""
+    s = torch.cuda.Stream()
+    cache = torch.zeros((2, 2, 1, ops.kv_tile_bytes(64, "int8")), dtype=torch.uint8, device="cuda")
+    q = torch.zeros((1, 4, 64), dtype=torch.float16, device="cuda")
+    pages, lens = i32(0).reshape(1, 1), i32(5)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    ops.release_workspace("cuda", s.cuda_stream)
+    with pytest.raises(RuntimeError, match="scratch"):
+        with torch.cuda.graph(g, stream=s):
+            ops.paged_attention(q, cache, pages, lens)
 
 
 # ---- together, streams, graphs -----------------------------------------------------------------------------------------------
