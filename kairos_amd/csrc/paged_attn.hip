@@ -1,15 +1,20 @@
 // Attention of one new token a sequence over the paged cache:
 //   o[b, h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q[b, h] . k_t - m),   t over the sequence's (window's) tokens
-// One pass over the cache with the running maximum m and sum of the softmax.  The G = H / KV query heads that share a key
+// One pass over the cache with a running reference m and sum of the softmax.  The G = H / KV query heads that share a key
 // head are the 16 columns of a matrix instruction, 32 tokens a step:
 //   S^T [token x head] = K Q^T      (16x16x32 MFMA, two row halves of 16 tokens)
 //   O^T [d x head]    += V^T P^T    (16x16x32 MFMA, a step's 32 tokens deep)
 // The cache's tile order makes the result registers of the first product, lane (head, g) = tokens 8 g .. 8 g + 7, the operand
-// registers of the second: nothing passes through LDS or between lanes but the maximum over the four lane groups.
+// registers of the second: nothing passes through LDS or between lanes but the maximum over the four lane groups, where m is raised.
 // Codes enter the products masked where they stand, as fp16 subnormals (the MFMA takes them exactly): one instruction for two.  A key's
-// factors meet its score in fp32, with the sum of q for the offset.  A value's scale multiplies p, relative to a running power of two
-// so that p stays normal in fp16; the middle of the codes is taken off the sums at the end by the sum of the same rounded weights (one
-// more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to one scalar a head.
+// factors meet its score in fp32, with the sum of q for the offset.  A value's scale multiplies p, in fp32 before the rounding to
+// fp16; m is one reference a head for p and for that product, so that both stay in range.  The codes' middle is taken off the sums at
+// the end by the sum of the same rounded weights (one more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to
+// one scalar a head.
+//
+// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 84-89 us for 435 MB, 4.9-5.2 TB/s (the same loads with no
+// arithmetic: 80 us); 2 x 131072 f16 (1074 MB) 182 us, 5.9 TB/s; 64 ragged up to 8192 f16 106 us, 5.2 TB/s; 32 x 1536 int8 20.0 us.  One
+// sequence of 200 tokens: 6.4 us, all of it latency (the schedule 2, the first loads 1, the joins 2).
 #include "kv_parts.h"
 
 // Waves of a workgroup, one workgroup a CU.  int4 tiles are small and cost as much vector work as the others: eight waves
@@ -27,6 +32,9 @@ static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start 
 // (64 x 62479 int8, 20 heads: 115 us against 176), but there are half as many shares (13 x up to 7411 int4: 21 us against 14).
 static constexpr long long PA_WIDE = 12288;
 
+// The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (4 x 100001 f16: off by 2.7e-4 of the
+// output's norm, 3.0e-4 with weights up to 1; rounding them costs 2e-4, the output's rounding another 2e-4).
+static constexpr float PA_LIFT = 8.0f;
 static constexpr float PA_NEG = -1e30f;       // running maximum before the first token: finite, so differences stay numbers
 
 // Over the four lane groups g that hold a head's tokens: the row swaps leave a pair of neighbouring groups' values in both.
@@ -63,15 +71,16 @@ __device__ __forceinline__ h8_t key_unit(const u4_t& c, int u) {
     return __builtin_bit_cast(h8_t, o);
 }
 
-// Value a (0 .. n - 1) of the eight tokens of a 16-byte value chunk: the element, or its code u as the subnormal u * 2^-24,
-// int4 with odd a u * 2^-20.
+// Value a (0 .. n - 1) of the eight tokens of a 16-byte value chunk: the element, or its code u as the subnormal u * 2^-24, for int4
+// u * 2^-20: measured, the sum of a product's terms loses low bits of subnormals (nibbles at 2^-24: outputs 3.6e-4 of their root mean
+// square too low over 100001 tokens, 1e-5 at 2^-20; bytes at 2^-24: 2e-5).
 template <int KIND>
 __device__ __forceinline__ h8_t value_unit(const u4_t& c, int a) {
     u4_t o = c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (KIND == KMI_KV_INT8) o[i] = a ? __builtin_amdgcn_perm(0u, c[i], 0x0C030C01u) : c[i] & 0x00FF00FFu;
-        if constexpr (KIND == KMI_KV_INT4) o[i] = (a & 2 ? c[i] >> 8 : c[i]) & (a & 1 ? 0x00F000F0u : 0x000F000Fu);
+        if constexpr (KIND == KMI_KV_INT4) o[i] = (a == 0 ? c[i] << 4 : c[i] >> (4 * a - 4)) & 0x00F000F0u;
     }
     return __builtin_bit_cast(h8_t, o);
 }
@@ -177,7 +186,7 @@ struct PaWave {
     }
     // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
     // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (to the largest x plus
-    // the logarithm of the largest value scale) only where a weight would pass 2^10 or p 2^40, which is seldom after a wave's
+    // the logarithm of the largest value scale) only where a weight would pass 2^15 or p 2^48, which is seldom after a wave's
     // first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
     // tokens that count, bad: no page of this cache.
     __device__ __forceinline__ h8_t weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
@@ -220,7 +229,7 @@ struct PaWave {
             wtop = fmaxf(wtop, wt[j]);
             if constexpr (CODES) ytop = fmaxf(ytop, y[j]);
         }
-        if (__any(wtop > 1024.0f || ytop > 40.0f)) {
+        if (__any(wtop > 32768.0f || ytop > 48.0f)) {
             float top = -__builtin_inff(), vtop = 0x1p-24f;
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
@@ -231,7 +240,7 @@ struct PaWave {
             }
             top = group_max(top);
             if constexpr (CODES) top += __builtin_amdgcn_logf(group_max(vtop));
-            const float m2 = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - m2);
+            const float m2 = fmaxf(m, top - PA_LIFT), a = __builtin_amdgcn_exp2f(m - m2);
             m = m2;
             l *= a; zsum *= a;
             if constexpr (CODES) psum = psum * a;
@@ -247,7 +256,7 @@ struct PaWave {
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             l += p[j];
-            if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(8.0f, vs[j], (float)fac.f[3][j]), zsum);
+            if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(7.5f, vs[j], (float)fac.f[3][j]), zsum);
             pf[j] = (half_t)wt[j];
         }
         if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
@@ -266,15 +275,15 @@ struct PaWave {
             psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w, psum, 0, 0, 0);
         }
     }
-    // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output -- the offsets,
-    // less the codes' middle times the very weights that entered the products, so that their rounding cancels.
+    // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output: the offsets (of the
+    // codes' middle), less the middle times the very weights that entered acc, so that their rounding cancels.
     __device__ __forceinline__ void totals(float& sum, float& add) const {
         sum = group_sum(l);
         add = 0.0f;
         if constexpr (KIND == KMI_KV_INT8) add = -128.0f * psum[0];
-        if constexpr (KIND == KMI_KV_INT4) add = group_sum(zsum) - 8.0f * psum[0];
+        if constexpr (KIND == KMI_KV_INT4) add = group_sum(zsum) - 7.5f * psum[0];
     }
-    static __device__ __forceinline__ float unit_of(int T) { return !CODES ? 1.0f : KIND == KMI_KV_INT4 && (T & 1) ? 0x1p20f : 0x1p24f; }
+    static constexpr float UNIT = !CODES ? 1.0f : KIND == KMI_KV_INT4 ? 0x1p20f : 0x1p24f;
     static __device__ __forceinline__ float other_half(float v) {          // row_ror 8: column c ^ 8 of the same lane group
         return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
     }
@@ -595,7 +604,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
                     for (int r = 0; r < 4; ++r) {
                         float y = o[r];
                         if constexpr (PACK == 2) y += W::other_half(y);
-                        if constexpr (W::CODES) y = __builtin_fmaf(y, W::unit_of(T), plus);
+                        if constexpr (W::CODES) y = __builtin_fmaf(y, W::UNIT, plus);
                         if ((PACK == 2 && col >= 8) || col + 16 * x >= used) continue;
                         const int d = W::d_of(T, 4 * g + r);
                         if (complete) out[(size_t)(col + 16 * x) * D + d] = (half_t)(y * norm);
