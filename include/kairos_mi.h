@@ -323,7 +323,7 @@ int kmi_kv_tile_bytes(int D, int kind);     /* bytes of a tile, or KMI_E_SHAPE; 
  * or (2i, 2i+1) with `interleaved`; rotary_dim 0 = no rotation.  Writes q_out (with q), k_out (if not NULL) and, with a
  * cache, the rotated keys and the values of the tokens' positions.  Tokens s >= count[b] (count may be NULL: none) are
  * padding: zeros in q_out / k_out, nothing in the cache.  q, k, v: fp16 [B][S][heads][D] with element strides for B and S
- * (multiples of 8), heads contiguous; outputs contiguous.  No two tokens of a call may share a place in the cache. */
+ * (multiples of 8), heads contiguous; outputs contiguous; S up to 2^26.  No two tokens of a call may share a place in the cache. */
 typedef struct {
     void* q_out;
     void* k_out;

@@ -277,6 +277,8 @@ def _rope_kv(what, q, k, v, start, table, interleaved, count, cache, page_table,
     dev = k.device
     kp, kb, kt = _need_rows(k, "k", what, dev)
     B, S, KV, D = k.shape
+    if KV == 0:
+        raise ValueError(f"{what}: k {tuple(k.shape)} has no heads")
     qp = qb = qt = vp = vb = vt = H = 0
     q_out = None
     if q is not None:

@@ -150,7 +150,7 @@ def _pack(form, base, change):
     (dict(H=70000), -2), (dict(rotary_dim=72), -2), (dict(rotary_dim=24), -2), (dict(rotary_dim=-16), -2), (dict(table=0), -2),
     (dict(table_rows=0), -2), (dict(kind=3), -2), (dict(kind=-1), -2), (dict(num_pages=0), -2), (dict(page_tiles=0), -2),
     (dict(max_pages=0), -2), (dict(max_pages=1 << 20, page_tiles=1 << 10), -2), (dict(max_pages=1 << 26), -2),
-    (dict(num_pages=1 << 28, KV=8), -2), (dict(B=0), 0), (dict(S=0), 0),
+    (dict(num_pages=1 << 28, KV=8), -2), (dict(S=(1 << 26) + 1), -2), (dict(B=0), 0), (dict(S=0), 0),
 ])
 def test_rope_kv_refusals(lib, change, code):
     from kairos_amd import ops
@@ -163,7 +163,7 @@ def test_rope_kv_refusals(lib, change, code):
 @pytest.mark.parametrize("change, code", [
     (dict(k_out=0), -1), (dict(v_out=0), -1), (dict(start=0), -1), (dict(cache=0), -1), (dict(page_table=0), -1), (dict(k_out=8), -5),
     (dict(cache=8), -5), (dict(D=32), -2), (dict(kind=4), -2), (dict(S=-1), -2), (dict(KV=0), -2), (dict(B=70000), -2),
-    (dict(num_pages=0), -2), (dict(max_pages=0), -2), (dict(S=0x7FFFFFFF, KV=65535), -2), (dict(B=0), 0), (dict(S=0), 0),
+    (dict(num_pages=0), -2), (dict(max_pages=0), -2), (dict(S=0x7FFFFFFF, KV=65535), -2), (dict(S=(1 << 26) + 1), -2), (dict(B=0), 0), (dict(S=0), 0),
 ])
 def test_kv_read_refusals(lib, change, code):
     from kairos_amd import ops

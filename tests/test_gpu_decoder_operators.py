@@ -674,6 +674,7 @@ def test_refusals(ops):
         (lambda: ops.kv_append(cache.transpose(0, 1), pages, start, k, k), ValueError), (lambda: ops.kv_append(cache, pages, start, k.cpu(), k), ValueError),
         (lambda: ops.kv_read(cache, pages, start, -1), ValueError), (lambda: ops.kv_read(cache, pages, start[:1], 3), ValueError),
         (lambda: ops.kv_read(cache, pages, start, 3, count=start.float()), TypeError),
+        (lambda: ops.rotary(q, k[:, :, :0], start, table), ValueError),          # nothing would turn q
         (lambda: ops.paged_attention(q[:, :2], cache, pages, start), ValueError), (lambda: ops.paged_attention(q[:, 0, :3], cache, pages, start), ValueError),
         (lambda: ops.paged_attention(q[:, 0], cache, pages, start, scale=0.0), Exception), (lambda: ops.paged_attention(q[:, 0], cache, pages, start, window=-1), Exception),
         (lambda: ops.paged_attention(q[:, 0], cache, pages, i32(1)), ValueError), (lambda: ops.paged_attention(q[:, 0].cpu(), cache, pages, start), ValueError),
