@@ -35,7 +35,7 @@ static constexpr long long PA_WIDE = 12288;
 // The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (4 x 100001 f16: off by 2.7e-4 of the
 // output's norm, 3.0e-4 with weights up to 1; rounding them costs 2e-4, the output's rounding another 2e-4).
 static constexpr float PA_LIFT = 8.0f;
-static constexpr float PA_NEG = -1e30f;       // running maximum before the first token: finite, so differences stay numbers
+static constexpr float PA_NEG = -1e30f;       // the reference before the first token: below every x, finite, so differences stay numbers
 
 // Over the four lane groups g that hold a head's tokens: the row swaps leave a pair of neighbouring groups' values in both.
 template <typename F>
@@ -185,9 +185,9 @@ struct PaWave {
         return __builtin_fmaf(s * c, (float)fac.f[0][j], __builtin_fmaf(qc, (float)fac.f[1][j], -less));
     }
     // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
-    // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (to the largest x plus
-    // the logarithm of the largest value scale) only where a weight would pass 2^15 or p 2^48, which is seldom after a wave's
-    // first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
+    // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (so that the largest weight
+    // is 2^8, or the largest p 2^40 where every value scale is tiny) only where a weight would pass 2^15 or p 2^48, which is seldom
+    // after a wave's first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
     // tokens that count, bad: no page of this cache.
     __device__ __forceinline__ h8_t weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
         float vs[NS], y[NS], p[NS], wt[NS];
@@ -230,17 +230,17 @@ struct PaWave {
             if constexpr (CODES) ytop = fmaxf(ytop, y[j]);
         }
         if (__any(wtop > 32768.0f || ytop > 48.0f)) {
-            float top = -__builtin_inff(), vtop = 0x1p-24f;
+            float top = -__builtin_inff(), wide = top;             // largest x, largest x + log2(value scale)
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 // from the products again: y is what m left of x
                 y[j] = y[j] == -__builtin_inff() ? y[j] : bad ? __builtin_nanf("") : exponent(sc.s[j], fac, j, 0.0f);
                 top = fmaxf(top, y[j]);
-                vtop = fmaxf(vtop, vs[j]);
+                if constexpr (CODES) wide = fmaxf(wide, y[j] + __builtin_amdgcn_logf(vs[j]));
             }
             top = group_max(top);
-            if constexpr (CODES) top += __builtin_amdgcn_logf(group_max(vtop));
-            const float m2 = fmaxf(m, top - PA_LIFT), a = __builtin_amdgcn_exp2f(m - m2);
+            const float m2 = fmaxf(m, CODES ? fmaxf(group_max(wide) - PA_LIFT, top - 40.0f) : top - PA_LIFT);
+            const float a = __builtin_amdgcn_exp2f(m - m2);
             m = m2;
             l *= a; zsum *= a;
             if constexpr (CODES) psum = psum * a;
@@ -655,8 +655,8 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
         return kmi_set_error(KMI_E_ALIGN, "%s: out, q and the workspace must be 16-byte aligned, q's stride a multiple of 8 elements", fn);
     const int rc = kv_check_cache(fn, p.cache, p.page_table, p.B, p.KV, p.D, p.kind, p.num_pages, p.page_tiles, p.max_pages);
     if (rc < 0) return rc;
-    if (p.H <= 0 || p.H % p.KV || p.H > 65535 || p.window < 0 || !(p.scale > 0.0f) || !(p.scale < 1e30f))
-        return kmi_set_error(KMI_E_SHAPE, "%s: need H a multiple of KV, window>=0 and a positive finite scale (H=%d KV=%d window=%d scale=%g)",
+    if (p.H <= 0 || p.H % p.KV || p.H > 65535 || p.window < 0 || !(p.scale > 0.0f) || !(p.scale < 1e16f))
+        return kmi_set_error(KMI_E_SHAPE, "%s: need H a multiple of KV, window>=0 and 0<scale<1e16, which no score leaves fp32 with (H=%d KV=%d window=%d scale=%g)",
                              fn, p.H, p.KV, p.window, (double)p.scale);
     if (p.B == 0) return KMI_OK;
     const long long pool = (long long)p.B * p.KV * p.max_pages * p.page_tiles;

@@ -174,7 +174,7 @@ def test_kv_read_refusals(lib, change, code):
 @pytest.mark.parametrize("change, code", [
     (dict(out=0), -1), (dict(q=0), -1), (dict(lens=0), -1), (dict(cache=0), -1), (dict(page_table=0), -1), (dict(out=8), -5), (dict(q=8), -5),
     (dict(q_batch=4), -5), (dict(H=5), -2), (dict(H=0), -2), (dict(KV=3), -2), (dict(D=80), -2), (dict(kind=9), -2), (dict(window=-1), -2),
-    (dict(scale=0.0), -2), (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(workspace=0), -2),
+    (dict(scale=0.0), -2), (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(scale=1e16), -2), (dict(workspace=0), -2),
     (dict(workspace_bytes=1 << 16), -2), (dict(workspace=8), -5), (dict(B=65535, KV=2, H=4, max_pages=1 << 20), -2), (dict(B=0), 0),
 ])
 def test_paged_attn_refusals(lib, change, code):

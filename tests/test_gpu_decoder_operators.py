@@ -296,6 +296,25 @@ def test_attention_sizes_of_values_and_scores(ops, size, qsize, kind):
     check_attention(ops, cache, pages, lens, q, 2, 64, kind)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H", [4, 12])
+def test_attention_small_values_beside_large_ones_without_weight(ops, H, kind):
+    """All weight on a token whose value is 1e-4, tokens with 60000 and a weight of e^-128 in its tile and the next: the small value's
+    weight keeps its 11 bits.  Off by its rounding and the output's, 2^-11 each of the row's largest, and half a subnormal step; the
+    codes' sums add 48 * 2^-24 of four times that."""
+    n, D = 40, 64
+    rng = np.random.default_rng(5)
+    cache, pages = random_cache(rng, 3, 1, 1, D, kind), np.array([[2, 0]], np.int32)
+    for t in range(n):
+        k = np.full(D, 4.0 if t == 5 else -4.0, np.float16)
+        v = (rng.standard_normal(D) * (1e-4 if t == 5 else 20000.0)).clip(-60000, 60000).astype(np.float16)
+        DO.put_token(cache[pages[0, t // 32], 0, 0], t % 32, k, v, kind)
+    q = np.full((1, H, D), 2.0, np.float16)
+    got = ops.paged_attention(dev(q), dev(cache), dev(pages), i32(n)).cpu().numpy().astype(np.float64)[0]
+    held = DO.sequence(cache, pages[0], n, 0, D, kind)[1][5].astype(np.float64)
+    assert np.abs(got - held).max() <= np.abs(held).max() * (2 * 2.0 ** -11 + 4 * 48 * 2.0 ** -24) + 2.0 ** -25
+
+
 def test_attention_strided_queries_and_4d(ops):
     rng = np.random.default_rng(2)
     lens = [70, 45]
