@@ -245,23 +245,31 @@ def _need_pages(page_table, batch, what, device):
     return page_table.data_ptr(), page_table.shape[1]
 
 
-def _need_rows(x, name, what, device):
-    """fp16 [B, S, heads, D] whose heads are contiguous; returns (pointer, batch stride, token stride) in elements."""
+def _need_rows(x, name, what, device, token=True):
+    """fp16 [B, S, heads, D], or [B, heads, D] without `token`, whose heads are contiguous; returns (pointer, batch stride, token
+    stride) in elements."""
     if x.dtype != torch.float16:
         raise TypeError(f"{name}: expected {torch.float16}, got {x.dtype}")
     if not x.is_cuda:
         raise ValueError(f"{name}: expected a GPU tensor (the HIP library is the only compute path)")
-    if x.dim() != 4 or x.device != device:
+    if x.dim() != (4 if token else 3) or x.device != device:
         raise ValueError(f"{what}: {name} must be fp16 [batch, tokens, heads, head_dim] on {device}, got {tuple(x.shape)} on {x.device}")
-    b, s, h, d = x.shape
-    sb, ss, sh, sd = x.stride()
-    if x.numel() == 0:
-        return x.data_ptr(), 0, 0
-    sb, ss = sb if b > 1 else 0, ss if s > 1 else 0
-    if (sd != 1 and d > 1) or (sh != d and h > 1) or (sb | ss) & 7 or x.data_ptr() & 15:
+    if token:
+        b, s, h, d = x.shape
+        sb, ss, sh, sd = x.stride()
+        if s <= 1:
+            ss = 0
+    else:
+        b, h, d = x.shape
+        sb, sh, sd = x.stride()
+        ss = 0
+    at = x.data_ptr()
+    if b <= 1:
+        sb = 0
+    if ((sd != 1 and d > 1) or (sh != d and h > 1) or (sb | ss) & 7 or at & 15) and x.numel():
         raise ValueError(f"{what}: {name}'s heads must lie behind each other, 16-byte aligned, at token and batch strides that are "
                          f"multiples of 8 elements; got strides {tuple(x.stride())} (call .contiguous())")
-    return x.data_ptr(), sb, ss
+    return at, sb, ss
 
 
 def _launch_on(device, name, M, N, K, fn, args):
@@ -366,24 +374,25 @@ def paged_attention(q, cache, page_table, lens, scale=None, window=0):
     D, kind = _cache_form(cache, "paged_attention")
     dev = cache.device
     if q.dim() == 3:
-        q4 = q.unsqueeze(1)
+        B, H, d = q.shape
+        qp, qb, _ = _need_rows(q, "q", "paged_attention", dev, token=False)
     elif q.dim() == 4 and q.shape[1] == 1:
-        q4 = q
+        B, _, H, d = q.shape
+        qp, qb, _ = _need_rows(q, "q", "paged_attention", dev)
     else:
         raise ValueError(f"paged_attention: q must be fp16 [batch, heads, head_dim] or [batch, 1, heads, head_dim], got {tuple(q.shape)}")
-    qp, qb, _ = _need_rows(q4, "q", "paged_attention", dev)
-    B, _, H, d = q4.shape
-    pages, KV, tiles = cache.shape[:3]
+    pages, KV, tiles, _ = cache.shape
     if d != D or H == 0 or H % KV:
         raise ValueError(f"paged_attention: q {tuple(q.shape)} does not fit a cache of {KV} heads of {D}")
     pp, width = _need_pages(page_table, B, "paged_attention", dev)
     lp = _need_index(lens, (B,), "lens", "paged_attention", dev)
     out = q.new_empty(q.shape)
     if B:
-        if dev.index != torch.cuda.current_device():
+        idx = torch.cuda.current_device()
+        if dev.index != idx:
             with torch.cuda.device(dev):
                 return paged_attention(q, cache, page_table, lens, scale, window)
-        st = _stream()
+        st = _raw_stream(idx) if _raw_stream is not None else _stream()
         ws = gemv_workspace_for(dev, st)
         try:
             _call("paged_attn", B, H, D, _lib.load().kmi_paged_attn, _paged_attn_args.pack(
