@@ -12,24 +12,42 @@
 // the end by the sum of the same rounded weights (one more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to
 // one scalar a head.
 //
-// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 84-89 us for 435 MB, 4.9-5.2 TB/s (the same loads with no
-// arithmetic: 80 us); 2 x 131072 f16 (1074 MB) 182 us, 5.9 TB/s; 64 ragged up to 8192 f16 106 us, 5.2 TB/s; 32 x 1536 int8 20.0 us.  One
-// sequence of 200 tokens: 6.4 us, all of it latency (the schedule 2, the first loads 1, the joins 2).
+// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 77 us for 435 MB, 5.6 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
+// 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.4 us, all of it latency (the
+// schedule 2, the first loads 1, the joins 2).
 #include "kv_parts.h"
 
-// Waves of a workgroup, one workgroup a CU.  int4 tiles are small and cost as much vector work as the others: eight waves
-// (two a SIMD, one computing while the other waits) read 4 x 100001 tokens in 84 us, four in 97; for int8 and f16 four read as fast (182
-// and 184 us for 2 x 131072 f16) and start and end a share sooner (32 x 1536 int8: 19.8 us against 20.3).
-static constexpr int pa_waves(int kind) { return kind == KMI_KV_INT4 ? 8 : 4; }
-// Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (182 us against 191 for 2 x 131072 f16: fewer places of
+// Waves of a workgroup.  Loads are short of flight where tiles are small, so there eight waves (two a SIMD, one computing while the other
+// waits): int4 (4 x 100001: 76 us, four waves 95), int8 with heads of 64 (8 x 60000: 84 us, 100), and 32 query heads a wave, for their
+// arithmetic (64 x 62479 int8, 20 heads: 91 us, 110).  Else four read as fast and start and end a share sooner (1 x 4096 int8:
+// 11.2 us, 13.6).  More tasks than CUs: small workgroups, several a CU, so that one task's end hides behind another's middle:
+// int4 of 128 with over 256 tasks four waves (64 x up to 1000, 8 key heads: 14 us, 30 with eight; up to 8000: 64, 79; but 256
+// tasks, 32 x 1536: 20, 14 with eight); from 2048 on, or 1024 of codes with heads of 64, two (256 x up to 300, 8 key heads of 128,
+// int8: 30 us, 40 with four; 1000 x up to 100 int4: 60, 83; against it 256 x up to 2000 f16: 184, 172).  Heads of 256 fill a SIMD's
+// registers with one wave.
+static constexpr bool pa_codes64(int D, int kind, int pack) { return kind != KMI_KV_F16 && D == 64 && pack == 2; }
+static int pa_waves(int D, int kind, int pack, int columns, long long tasks) {
+    if (columns == 32) return 8;
+    if (D < 256 && tasks >= (pa_codes64(D, kind, pack) ? 1024 : 2048)) return 2;
+    if (pa_codes64(D, kind, pack)) return 8;
+    return kind == KMI_KV_INT4 && (D == 256 || tasks <= 256) ? 8 : 4;
+}
+static constexpr int pa_a_cu(int D, int kind, int pack, int waves) {         // workgroups that fit a CU's registers
+    const int most = D == 256 ? 4 : pa_codes64(D, kind, pack) ? 16 : kind == KMI_KV_INT4 && pack == 2 ? 12 : 8;      // waves
+    return most < waves ? 1 : most / waves;
+}
+// Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (161 us against 169 for 2 x 131072 f16: fewer places of
 // memory at once), 512 hide the starts and ends of short tasks (19 sequences of up to 7985, int8, 64 wide: 20 us against 29).
 static constexpr int PA_LONG = 96;            // tiles a share from which 256 uneven ones are taken all the same
 // Being cut costs a task about 3 us (hand-off and join): none of up to nine tiles a wave is (2 x 1152 f16, 36 tiles: 9.6 us
 // whole, 10.6 cut), and no share is smaller than three (1 x 4096 f16: 11.8 us, 13.2 with six).
 static constexpr int PA_WHOLE_STEPS = 9, PA_MIN_STEPS = 3;
+static constexpr int PA_SMALL_BYTES = 320 << 10;   // of a task that no row of tasks is cut in (256 x up to 300 f16: 42 us, 46 with such cuts)
+static constexpr int PA_HELD = 1024;          // sequences whose lengths the schedule keeps in LDS
 static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start and end; 3 and 12 measured the same
-// Tiles of the page table from which a wave takes 32 query heads at once (more than 16 share a key head): the cache is read once
-// (64 x 62479 int8, 20 heads: 115 us against 176), but there are half as many shares (13 x up to 7411 int4: 21 us against 14).
+// Tiles of the page table from which a wave takes 32 query heads at once (more than 16 share a key head; not int4, whose arithmetic
+// then spills: 40 us against 30): the cache is read once (16 x up to 20000 f16, 64 heads on 2: 43 us against 63; int8 33 and 40), but
+// there are half as many shares (13 x up to 7411 int4: 21 us against 14).
 static constexpr long long PA_WIDE = 12288;
 
 // The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (4 x 100001 f16: off by 2.7e-4 of the
@@ -147,15 +165,17 @@ struct PaWave {
     // The first of the lane's NS tokens in a tile.
     static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
 
+    // A cache is read once a step: loads that leave nothing behind in the caches (2 x 131072 f16: 161 us, 182 with ordinary ones; 64 ragged up
+    // to 8192: 93, 107; against it a cache small enough to stay: 8 x up to 3000 f16, heads of 256: 27, 20).
     static __device__ __forceinline__ void load_keys(Tile& t, const char* tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) t.k[i] = *reinterpret_cast<const u4_t*>(tile + i * 1024 + lane * 16);
+        for (int i = 0; i < CH; ++i) t.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(tile + i * 1024 + lane * 16));
 #pragma unroll
         for (int i = 0; i < NF; ++i) t.f.f[i] = *reinterpret_cast<const fac_t*>(tile + 2 * PART + 64 * i + 2 * first_token(lane));
     }
     static __device__ __forceinline__ void load_values(Tile& t, const char* tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) t.v[i] = *reinterpret_cast<const u4_t*>(tile + PART + i * 1024 + lane * 16);
+        for (int i = 0; i < CH; ++i) t.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(tile + PART + i * 1024 + lane * 16));
     }
 
     // Raw scores of the lane's tokens and column.
@@ -429,9 +449,9 @@ __device__ __forceinline__ void join_shares(const float* partial, int slot, int 
     }
 }
 
-template <int D, int KIND, int PACK, int HT>
-__global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 256 ? 1 : 2) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
-    constexpr int NW = pa_waves(KIND), MINE = D / 16 / NW > 0 ? D / 16 / NW : 1;         // MINE: output tiles that a wave joins
+template <int D, int KIND, int PACK, int HT, int NW>
+__global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void paged_attn_kernel(kmi_paged_attn_args p, PaSplit sp) {
+    constexpr int MINE = D / 16 / NW > 0 ? D / 16 / NW : 1;         // MINE: output tiles that a wave joins
     using W = PaWave<D, KIND, PACK>;
     __shared__ PaJoin<D, NW> join;
     __shared__ int last;
@@ -439,10 +459,16 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
     const int G = p.H / p.KV, run = blockIdx.x;
     half_t* out0 = static_cast<half_t*>(p.out);
 
+    __shared__ int held_lens[PA_HELD];
     const int lens0 = lane < p.B ? p.lens[lane] : 0;                       // of the first 64 sequences: most often all
+    if (p.B > 64) {
+        for (int b = threadIdx.x; b < min(p.B, PA_HELD); b += 64 * NW) held_lens[b] = p.lens[b];
+        __syncthreads();
+    }
+    auto length = [&](int b) { return b < PA_HELD ? held_lens[b] : p.lens[b]; };
     auto tiles_of = [&](int b0) {                                          // of sequence b0 + lane
         const int b = b0 + lane;
-        return b < p.B ? pa_sequence(p, b0 == 0 ? lens0 : p.lens[b]).tiles : 0;
+        return b < p.B ? pa_sequence(p, b0 == 0 ? lens0 : length(b)).tiles : 0;
     };
     auto sum_over = [&](auto f) {                                          // over the sequences, f(tiles), times the tasks of one
         int v = 0;
@@ -454,7 +480,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
     auto quota_of = [&](int units, int shares) { return (max((units + shares - 1) / shares, PA_MIN_STEPS * NW) + NW - 1) / NW * NW; };
     auto pieces_of = [](int n, int q) { return n <= PA_WHOLE_STEPS * NW ? (n > 0 ? 1 : 0) : (n + q - 1) / q; };
     auto pieces = [&](int q) { return sum_over([&](int n) { return pieces_of(n, q); }); };
-    int shares = min(most, 256), quota = quota_of(units, shares);
+    int shares = NW == 2 || (KIND == KMI_KV_INT4 && NW == 4) ? most : min(most, 256), quota = quota_of(units, shares);
     bool even = pieces(quota) <= shares;
     for (int pass = 0; !even; ++pass) {
         const int more = (quota + quota / 8 + NW - 1) / NW * NW;
@@ -472,6 +498,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
     }
     // the row that the shares are cut from: pieces, one a share, or tiles and PA_TASK_COST a task, `quota` a share
     auto room = [&](int n) { return n == 0 ? 0 : even ? pieces_of(n, quota) : n + PA_TASK_COST; };     // a task's, in the row
+    constexpr int SMALL = PA_WHOLE_STEPS * NW < PA_SMALL_BYTES / W::TILE_BYTES ? PA_WHOLE_STEPS * NW : PA_SMALL_BYTES / W::TILE_BYTES;
     const int per_share = even ? 1 : quota, begin = run * per_share, end = begin + per_share;
     int b = p.B, before = 0;                                               // before: the room of the sequences in front
     for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -485,7 +512,7 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    auto len_of = [&](int b) { return b < 64 ? __builtin_amdgcn_readlane(lens0, b & 63) : p.lens[b]; };
+    auto len_of = [&](int b) { return b < 64 ? __builtin_amdgcn_readlane(lens0, b & 63) : __builtin_amdgcn_readfirstlane(length(b)); };
 
     for (int unit = begin; unit < end && b < p.B;) {
         const PaSequence seq = pa_sequence(p, len_of(b));
@@ -503,6 +530,12 @@ __global__ __launch_bounds__(64 * pa_waves(KIND), pa_waves(KIND) == 8 || D == 25
             tb = (int)((long)(ta + 1) * seq.tiles / space);
             ta = (int)((long)ta * seq.tiles / space);
             unit = end;
+        } else if (seq.tiles <= SMALL) {
+            const int middle = task0 + space / 2;
+            unit = task0 + space;
+            if (middle < begin || middle >= end) continue;
+            ta = 0;
+            tb = seq.tiles;
         } else {
             tb = min(seq.tiles, end - task0);
             unit = task0 + min(space, end - task0);
@@ -660,7 +693,7 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
                              fn, p.H, p.KV, p.window, (double)p.scale);
     if (p.B == 0) return KMI_OK;
     const long long pool = (long long)p.B * p.KV * p.max_pages * p.page_tiles;
-    const int G = p.H / p.KV, columns = G > 16 && p.D < 256 && pool >= PA_WIDE ? 32 : 16, used = G < columns ? G : columns;
+    const int G = p.H / p.KV, columns = G > 16 && p.D < 256 && p.kind != KMI_KV_INT4 && pool >= PA_WIDE ? 32 : 16, used = G < columns ? G : columns;
     PaSplit sp;
     sp.head_tiles = (G + columns - 1) / columns;
     sp.tasks_a_sequence = p.KV * sp.head_tiles;
@@ -673,26 +706,45 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* args, void* stream) {
     if (most > 0x7FFF0000ll)
         return kmi_set_error(KMI_E_SHAPE, "%s: %d sequences of %d pages hold more than 2^31 tiles", fn, p.B, p.max_pages);
     const long long pieces = (long long)p.B * sp.tasks_a_sequence * (((long long)p.max_pages * p.page_tiles + 7) / 8);
-    const int waves = pa_waves(p.kind), most_runs = waves == 8 ? 256 : 512, runs = (int)(pieces < most_runs ? pieces : most_runs);
+    const int pack = G > 8 || p.kind == KMI_KV_F16 ? 1 : 2, waves = pa_waves(p.D, p.kind, pack, columns, (long long)p.B * sp.tasks_a_sequence);
+    const int most_runs = 256 * pa_a_cu(p.D, p.kind, pack, waves), runs = (int)(pieces < most_runs ? pieces : most_runs);
     const size_t need = KMI_GEMV_WS_HEADER + (size_t)most_runs * 2 * sp.slot * sizeof(float);
     if (!p.workspace || p.workspace_bytes < need)
         return kmi_set_error(KMI_E_SHAPE, "%s: the workspace must hold %zu bytes (has %zu)", fn, need, p.workspace ? (size_t)p.workspace_bytes : (size_t)0);
     const dim3 grid(runs), block(waves * 64);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define KMI_PA_KIND(D_, K_)                                                                                                     \
-    if (columns == 32) hipLaunchKernelGGL((paged_attn_kernel<D_, K_, 1, D_ == 256 ? 1 : 2>), grid, block, 0, st, p, sp);        \
-    else if (G > 8 || K_ == KMI_KV_F16) hipLaunchKernelGGL((paged_attn_kernel<D_, K_, 1, 1>), grid, block, 0, st, p, sp);       \
-    else hipLaunchKernelGGL((paged_attn_kernel<D_, K_, K_ == KMI_KV_F16 ? 1 : 2, 1>), grid, block, 0, st, p, sp)
-#define KMI_PA_LAUNCH(D_)                                          \
-    switch (p.kind) {                                              \
-        case KMI_KV_F16: KMI_PA_KIND(D_, KMI_KV_F16); break;       \
-        case KMI_KV_INT8: KMI_PA_KIND(D_, KMI_KV_INT8); break;     \
-        default: KMI_PA_KIND(D_, KMI_KV_INT4);                     \
+#define KMI_PA(D_, K_, PACK_, HT_, NW_) hipLaunchKernelGGL((paged_attn_kernel<D_, K_, PACK_, HT_, NW_>), grid, block, 0, st, p, sp)
+#define KMI_PA_WAVES(D_, K_, PACK_, NW_)                                             \
+    if (D_ < 256 && waves == 2) KMI_PA(D_, K_, PACK_, 1, D_ == 256 ? NW_ : 2);       \
+    else KMI_PA(D_, K_, PACK_, 1, NW_)
+#define KMI_PA_WIDE(D_, K_) if (D_ < 256 && columns == 32) KMI_PA(D_, K_, 1, D_ == 256 ? 1 : 2, D_ == 256 ? 4 : 8)
+#define KMI_PA_F16(D_)                                             \
+    KMI_PA_WIDE(D_, KMI_KV_F16);                                   \
+    else KMI_PA_WAVES(D_, KMI_KV_F16, 1, 4)
+#define KMI_PA_INT8(D_)                                            \
+    KMI_PA_WIDE(D_, KMI_KV_INT8);                                  \
+    else if (pack == 1) { KMI_PA_WAVES(D_, KMI_KV_INT8, 1, 4); }   \
+    else KMI_PA_WAVES(D_, KMI_KV_INT8, 2, D_ == 64 ? 8 : 4)
+#define KMI_PA_INT4(D_)                                                                   \
+    if (pack == 1 && waves == 8) KMI_PA(D_, KMI_KV_INT4, 1, 1, 8);                        \
+    else if (pack == 1) { KMI_PA_WAVES(D_, KMI_KV_INT4, 1, D_ == 256 ? 8 : 4); }          \
+    else if (waves == 8) KMI_PA(D_, KMI_KV_INT4, 2, 1, 8);                                \
+    else KMI_PA_WAVES(D_, KMI_KV_INT4, 2, D_ == 128 ? 4 : 8)
+#define KMI_PA_LAUNCH(D_)                                  \
+    switch (p.kind) {                                      \
+        case KMI_KV_F16: KMI_PA_F16(D_); break;            \
+        case KMI_KV_INT8: KMI_PA_INT8(D_); break;          \
+        default: KMI_PA_INT4(D_);                          \
     }
     if (p.D == 64) { KMI_PA_LAUNCH(64) }
     else if (p.D == 128) { KMI_PA_LAUNCH(128) }
     else { KMI_PA_LAUNCH(256) }
 #undef KMI_PA_LAUNCH
-#undef KMI_PA_KIND
+#undef KMI_PA_INT4
+#undef KMI_PA_INT8
+#undef KMI_PA_F16
+#undef KMI_PA_WIDE
+#undef KMI_PA_WAVES
+#undef KMI_PA
     return kmi_check_launch(fn);
 }

@@ -407,6 +407,27 @@ def test_attention_work_shared_out(ops, B, KV, lens, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, G, B, KV", [(128, 4, 40, 8), (128, 12, 40, 8), (64, 12, 40, 8), (64, 4, 135, 8), (128, 4, 260, 8), (64, 3, 260, 8), (128, 12, 130, 16),
+                                         (64, 12, 130, 16), (256, 2, 130, 16), (64, 1, 1100, 2)])
+def test_attention_of_many_tasks(ops, D, G, B, KV, kind):
+    """From a task more than CUs up to many thousands, short ones, none, and one so long that it is cut among them; over 1024 lengths."""
+    lens = [0 if i % 9 == 4 else 700 if i == 17 else 1 + (i * 23) % 45 for i in range(B)]
+    rng = np.random.default_rng(B + G)
+    cache, pages = appended(ops, rng, lens, KV, D, kind, 32)
+    q = (rng.standard_normal((B, G * KV, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    again = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    host = cache.cpu().numpy()
+    some = [4, 17, B // 2, B - 1]
+    check_attention(ops, host, pages[some], [lens[b] for b in some], q[some], KV, D, kind, got=got[some])
+    # the others against the same sequences shared out differently: twice (|o| + mean |v|) 2^-11 with |v| < 6, 2^-6.4, and as much for scores and codes
+    for at in range(0, B, 64):
+        part = ops.paged_attention(dev(q[at:at + 64]), cache, dev(pages[at:at + 64]), i32(*lens[at:at + 64]))
+        assert (part.float() - got[at:at + 64].float()).abs().max() <= 2.0 ** -5
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D, G", [(64, 17), (64, 32), (64, 33), (128, 20), (128, 64), (256, 20)])
 def test_attention_many_heads_on_a_wide_page_table(ops, D, G, kind):
     """Page tables with room for far longer sequences: 32 query heads at once where more than 16 share a key head, one sequence cut."""
