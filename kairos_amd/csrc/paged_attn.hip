@@ -37,7 +37,7 @@ static constexpr int pa_a_cu(int D, int kind, int pack, int waves) {         // 
     return most < waves ? 1 : most / waves;
 }
 // Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (161 us against 169 for 2 x 131072 f16: fewer places of
-// memory at once), 512 hide the starts and ends of short tasks (19 sequences of up to 7985, int8, 64 wide: 20 us against 29).
+// memory at once), more hide the starts and ends of short tasks (64 x up to 1000 int8, 8 key heads: 18.5 us, 29 with 256 workgroups).
 static constexpr int PA_LONG = 96;            // tiles a share from which 256 uneven ones are taken all the same
 // Being cut costs a task about 3 us (hand-off and join): none of up to nine tiles a wave is (2 x 1152 f16, 36 tiles: 9.6 us
 // whole, 10.6 cut), and no share is smaller than three (1 x 4096 f16: 11.8 us, 13.2 with six).
