@@ -12,7 +12,7 @@
 // the end by the sum of the same rounded weights (one more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to
 // one scalar a head.
 //
-// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 77 us for 435 MB, 5.6 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
+// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 74-77 us for 435 MB, 5.7-5.9 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
 // 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.4 us, all of it latency (the
 // schedule 2, the first loads 1, the joins 2).
 #include "kv_parts.h"
