@@ -428,6 +428,23 @@ def test_attention_of_many_tasks(ops, D, G, B, KV, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, G, B, KV, width", [(128, 16, 1, 1, 1), (128, 16, 130, 16, 2), (64, 16, 130, 16, 2), (64, 8, 130, 16, 2), (128, 8, 40, 8, 2), (256, 16, 2, 2, 1), (128, 32, 16, 2, 400)])
+def test_the_stated_workspace_suffices(ops, D, G, B, KV, width, kind):
+    """64 KiB of counters and 17 MiB, as the header says, for whatever share of the work the shape asks for; counters left zero."""
+    from kairos_amd import _lib
+    cache = torch.zeros((4, KV, 1, ops.kv_tile_bytes(D, kind)), dtype=torch.uint8, device="cuda")
+    pages, lens = torch.ones((B, width), dtype=torch.int32, device="cuda"), torch.full((B,), 32 * width, dtype=torch.int32, device="cuda")
+    q = torch.ones((B, G * KV, D), dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ws = torch.zeros(65536 + (17 << 20), dtype=torch.uint8, device="cuda")
+    args = ops._paged_attn_args.pack(out.data_ptr(), q.data_ptr(), cache.data_ptr(), pages.data_ptr(), lens.data_ptr(), ws.data_ptr(), ws.numel(),
+                                     G * KV * D, 0.1, B, G * KV, KV, D, ops.KV_KINDS[kind], 4, 1, width, 0)
+    assert _lib.load().kmi_paged_attn(args, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert not out.any() and not ws[:65536].any()              # a cache of zeros: int8 stands for 0 * (0 - 128)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D, G", [(64, 17), (64, 32), (64, 33), (128, 20), (128, 64), (256, 20)])
 def test_attention_many_heads_on_a_wide_page_table(ops, D, G, kind):
     """Page tables with room for far longer sequences: 32 query heads at once where more than 16 share a key head, one sequence cut."""
