@@ -232,7 +232,7 @@ def _cache_form(cache, what):
 
 def _need_index(t, shape, name, what, device):
     _need(t, torch.int32, name)
-    if tuple(t.shape) != shape or t.device != device:
+    if t.shape != shape or t.device != device:
         raise ValueError(f"{what}: {name} must be int32 {list(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -287,34 +287,38 @@ def _rope_kv(what, q, k, v, start, table, interleaved, count, cache, page_table,
     B, S, KV, D = k.shape
     if KV == 0:
         raise ValueError(f"{what}: k {tuple(k.shape)} has no heads")
-    qp = qb = qt = vp = vb = vt = H = 0
+    qp = qb = qt = vp = vb = vt = H = qo = 0
     q_out = None
     if q is not None:
         qp, qb, qt = _need_rows(q, "q", what, dev)
-        H = q.shape[2]
-        if q.shape[:2] != k.shape[:2] or q.shape[3] != D or H == 0:
+        qB, qS, H, qD = q.shape
+        if qB != B or qS != S or qD != D or H == 0:
             raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head_dim")
         q_out = q.new_empty((B, S, H, D))
+        qo = q_out.data_ptr()
     cp = kind = pages = tiles = pp = width = 0
     if cache is not None:
         cd, kind = _cache_form(cache, what)
         vp, vb, vt = _need_rows(v, "v", what, dev)
-        if v.shape != k.shape or cd != D or cache.shape[1] != KV or cache.device != dev:
+        pages, heads, tiles, _ = cache.shape
+        if v.shape != k.shape or cd != D or heads != KV or cache.device != dev:
             raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the cache {tuple(cache.shape)} "
                              f"(head_dim {cd}) on {cache.device}")
         pp, width = _need_pages(page_table, B, what, dev)
-        cp, pages, tiles = cache.data_ptr(), cache.shape[0], cache.shape[2]
+        cp = cache.data_ptr()
     tp = R = rows = 0
     if table is not None:
         _need(table, torch.float32, "table")
         if table.dim() != 3 or table.shape[2] != 2 or table.device != dev:
             raise ValueError(f"{what}: table must be fp32 [positions, rotary_dim / 2, 2] on {dev}, got {tuple(table.shape)} on {table.device}")
-        tp, rows, R = table.data_ptr(), table.shape[0], 2 * table.shape[1]
+        tp = table.data_ptr()
+        rows, R, _ = table.shape
+        R *= 2
     sp = _need_index(start, (B,), "start", what, dev)
     np_ = 0 if count is None else _need_index(count, (B,), "count", what, dev)
-    if k.numel():
+    if B and S:
         _launch_on(dev, "rope_kv", B * S, H + KV, D, _lib.load().kmi_rope_kv, _rope_kv_args.pack(
-            _ptr(q_out), _ptr(k_out), cp, qp, kp, vp, tp, sp, np_, pp, qb, qt, kb, kt, vb, vt,
+            qo, _ptr(k_out), cp, qp, kp, vp, tp, sp, np_, pp, qb, qt, kb, kt, vb, vt,
             B, S, H, KV, D, R, rows, 1 if interleaved else 0, kind, pages, tiles, width))
     return q_out
 
