@@ -13,7 +13,7 @@
 // one scalar a head.
 //
 // Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 74-77 us for 435 MB, 5.7-5.9 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
-// 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.4 us, all of it latency (the
+// 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.5 us, all of it latency (the
 // schedule 2, the first loads 1, the joins 2).
 #include "kv_parts.h"
 
@@ -50,8 +50,8 @@ static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start 
 // there are half as many shares (13 x up to 7411 int4: 21 us against 14).
 static constexpr long long PA_WIDE = 12288;
 
-// The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (4 x 100001 f16: off by 2.7e-4 of the
-// output's norm, 3.0e-4 with weights up to 1; rounding them costs 2e-4, the output's rounding another 2e-4).
+// The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (int8 and int4 over 4 x 100001 tokens off
+// by 2.3e-4 of the output's norm, the output's own rounding 2.1e-4).
 static constexpr float PA_LIFT = 8.0f;
 static constexpr float PA_NEG = -1e30f;       // the reference before the first token: below every x, finite, so differences stay numbers
 
@@ -162,6 +162,11 @@ struct PaWave {
     struct Scores {
         float s[NS];
     };
+    // f16: the weights in two numbers of fp16, 22 bits, so that nothing but the output is rounded to 11 (off by 2.1e-4 of the output's
+    // norm, 2.7e-4 with one, in the same time: 2 x 131072 162 us); codes, whose arithmetic is dearer, in one (2.2e-4 to 2.5e-4).
+    struct Weights {
+        h8_t high, low;
+    };
     // The first of the lane's NS tokens in a tile.
     static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
 
@@ -204,12 +209,12 @@ struct PaWave {
         if constexpr (KIND == KMI_KV_INT8) return __builtin_fmaf(__builtin_fmaf(s, c, -128.0f * qc), (float)fac.f[0][j], -less);
         return __builtin_fmaf(s * c, (float)fac.f[0][j], __builtin_fmaf(qc, (float)fac.f[1][j], -less));
     }
-    // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as the fp16
-    // operand; the reference, the sums and the accumulators are brought to them.  The reference is raised (so that the largest weight
+    // The weights that meet the values -- p, for codes p times the token's value scale -- from the products' results, as fp16
+    // operands; the reference, the sums and the accumulators are brought to them.  The reference is raised (so that the largest weight
     // is 2^8, or the largest p 2^40 where every value scale is tiny) only where a weight would pass 2^15 or p 2^48, which is seldom
     // after a wave's first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
     // tokens that count, bad: no page of this cache.
-    __device__ __forceinline__ h8_t weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
+    __device__ __forceinline__ Weights weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
         float vs[NS], y[NS], p[NS], wt[NS];
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -272,27 +277,31 @@ struct PaWave {
                 wt[j] = CODES ? p[j] * vs[j] : p[j];
             }
         }
-        h8_t pf = {};
+        h8_t pf = {}, rest = {};
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             l += p[j];
             if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(7.5f, vs[j], (float)fac.f[3][j]), zsum);
             pf[j] = (half_t)wt[j];
+            if constexpr (!CODES) rest[j] = (half_t)(wt[j] - (float)pf[j]);
         }
         if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
             const u4_t w = __builtin_bit_cast(u4_t, pf);
             const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
             pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
         }
-        return pf;
+        return {pf, rest};
     }
-    __device__ __forceinline__ void add(const Tile& tile, const h8_t& w) {
+    __device__ __forceinline__ void add(const Tile& tile, const Weights& w) {
 #pragma unroll
-        for (int T = 0; T < OT; ++T)
-            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value_unit<KIND>(tile.v[T / n], T % n), w, acc[T], 0, 0, 0);
+        for (int T = 0; T < OT; ++T) {
+            const h8_t v = value_unit<KIND>(tile.v[T / n], T % n);
+            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.high, acc[T], 0, 0, 0);
+            if constexpr (!CODES) acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.low, acc[T], 0, 0, 0);
+        }
         if constexpr (CODES) {
             const half_t one = (half_t)1.0f;
-            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w, psum, 0, 0, 0);
+            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w.high, psum, 0, 0, 0);
         }
     }
     // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output: the offsets (of the
@@ -586,7 +595,7 @@ __global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void 
             const bool bad = place < 0;
             if constexpr (more.value) fetch_keys(i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            h8_t o[HT];
+            typename W::Weights o[HT];
 #pragma unroll
             for (int x = 0; x < HT; ++x)
                 o[x] = w[x].weights(sc[x], tile, fac, (seq.first + ta + wave + NW * i) * KV_TILE, seq.lo, seq.hi, bad, lane);
