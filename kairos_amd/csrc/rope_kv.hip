@@ -11,7 +11,7 @@
 // once: the codes are the same on any machine.  A row with an infinity or NaN gets the scale NaN and reads as NaN.
 // Traffic: every row read once and written once, plus the table's R * 4 bytes a token; bound by the memory.  Measured: rotation
 // alone, 4 x 4001 tokens, 28 + 4 heads of 128: 50 us for 262 MB, 5.2 TB/s (a large copy: 5.0); into the cache, 32 x 1024 tokens, 32 + 8 + 8
-// heads of 128: int4 158 us for 707 MB, 4.5 TB/s; 3 x 777 tokens, 64 + 8 + 8 heads, f16: 23 us for 95 MB, 4.1 TB/s; one token of 32 sequences: 4 us.
+// heads of 128: int4 158 us for 707 MB, 4.5 TB/s; 3 x 777 tokens, 64 + 8 + 8 heads, f16: 22 us for 96 MB, 4.4 TB/s; one token of 32 sequences: 4 us.
 #include "kv_parts.h"
 #include <type_traits>
 
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
     if (r >= p.H + p.KV + (KIND >= 0 ? p.KV : 0)) return;
     const bool is_q = r < p.H, is_v = r >= p.H + p.KV;
     const int head = is_q ? r : is_v ? r - p.H - p.KV : r - p.H;
-    const int start = p.start[b], count = p.count ? min(p.count[b], p.S) : p.S;
+    const int start = p.start[b], count = p.count ? max(0, min(p.count[b], p.S)) : p.S;
     const int pos0 = (int)((unsigned)((start >> 3) + (int)blockIdx.x) << 3), s0 = (int)((unsigned)pos0 - (unsigned)start);
     if (s0 >= p.S) return;
 
@@ -337,18 +337,17 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
         }
         return;
     }
-    for (int j = 0; j < 8; ++j) {
-        const int s = s0 + j;
-        if (s < 0 || s >= p.S) continue;
-        if (s >= count) {                                       // rows behind the sequence: zeros out, nothing into the cache
-            if (out) { store(s, at.da, h8_t{}); store(s, at.db, h8_t{}); }
-            continue;
+    const int lo = max(0, -s0), hi = min(8, count - s0);       // the tokens that are there
+    if (out) {
+        for (int j = max(lo, hi); j < 8 && s0 + j < p.S; ++j) { // rows behind the sequence: zeros out, nothing into the cache
+            store(s0 + j, at.da, h8_t{});
+            store(s0 + j, at.db, h8_t{});
         }
-        h8_t xa = load(s, at.da), xb = load(s, at.db);
-        if (!is_v) turn(xa, xb, table, p.table_rows, R, pos0 + j, at);
-        if (out) { store(s, at.da, xa); store(s, at.db, xb); }
+    }
+    auto put = [&](int j, h8_t xa, h8_t xb) {
+        if (out) { store(s0 + j, at.da, xa); store(s0 + j, at.db, xb); }
         if constexpr (KIND >= 0) {
-            if (!tile) continue;
+            if (!tile) return;
             const RowFactors f = row_factors<LPR, K_>(xa, xb);
             const Packed<K_> wa = pack_row<K_>(xa, f), wb = pack_row<K_>(xb, f);
             if (is_v) {
@@ -360,6 +359,28 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(kmi_rope_kv_args p) {
             }
             if (c == 0) store_factors<D, K_>(tile, tau0 + j, is_v ? kv_factors(K_) / 2 : 0, f);
         }
+    };
+    if (hi <= lo) return;
+    if (hi == lo + 1) {                                         // a decode step
+        h8_t xa = load(s0 + lo, at.da), xb = load(s0 + lo, at.db);
+        if (!is_v) turn(xa, xb, table, p.table_rows, R, pos0 + lo, at);
+        put(lo, xa, xb);
+        return;
+    }
+    // a few: one after the other, each would wait for its own loads; so eight are loaded and turned, some of them twice
+    h8_t xa[8], xb[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int there = min(max(j, lo), hi - 1);
+        xa[j] = load(s0 + there, at.da); xb[j] = load(s0 + there, at.db);
+    }
+    if (!is_v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) turn(xa[j], xb[j], table, p.table_rows, R, pos0 + min(max(j, lo), hi - 1), at);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (j >= lo && j < hi) put(j, xa[j], xb[j]);
     }
 }
 

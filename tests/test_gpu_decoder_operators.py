@@ -157,6 +157,25 @@ def test_append_writes_the_oracle_s_bytes_and_read_returns_them(ops, S, page, st
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [-2 ** 31, -1, 0, 1, 2, 7, 2 ** 31 - 1])
+def test_append_of_any_count(ops, count, kind):
+    """Counts from the least to the largest int32, starts that leave one or a few tokens in the first group of eight: the tokens that are
+    there stand in the cache as if appended one by one, the others come back as zeros and leave the cache as it was."""
+    B, S, H, KV, D = 3, 19, 4, 2, 64
+    rng = np.random.default_rng(6)
+    q, k, v = (dev(rng.standard_normal((B, S, n, D)).astype(np.float16)) for n in (H, KV, KV))
+    pages, start = i32(*range(6)).reshape(3, 2), i32(7, 6, 2)
+    table = torch.from_numpy(rng.standard_normal((64, D // 2, 2)).astype(np.float32)).cuda()
+    both = [torch.full((6, KV, 1, ops.kv_tile_bytes(D, kind)), 9, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    got, turned = ops.kv_append(both[0], pages, start, k, v, table, q=q, count=i32(count, count, count), want_k=True)
+    there = min(max(count, 0), S)
+    for s in range(there):
+        one, k1 = ops.kv_append(both[1], pages, start + s, k[:, s:s + 1], v[:, s:s + 1], table, q=q[:, s:s + 1], want_k=True)
+        assert torch.equal(got[:, s:s + 1], one) and torch.equal(turned[:, s:s + 1], k1)
+    assert torch.equal(both[0], both[1]) and not got[:, there:].any() and not turned[:, there:].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_pages_outside_the_cache_are_never_followed(ops, kind):
     """Entries of -1, of the pool's size and of 2^31 - 1, and positions past the row of the page table: writes are dropped, reads give
     NaN, neighbours are untouched."""
