@@ -6,11 +6,12 @@
 //   O^T [d x head]    += V^T P^T    (16x16x32 MFMA, a step's 32 tokens deep)
 // The cache's tile order makes the result registers of the first product, lane (head, g) = tokens 8 g .. 8 g + 7, the operand
 // registers of the second: nothing passes through LDS or between lanes but the maximum over the four lane groups, where m is raised.
+// The weights enter the second product as two fp16 numbers that add up to 22 bits, an instruction each.
 // Codes enter the products masked where they stand, as fp16 subnormals (the MFMA takes them exactly): one instruction for two.  A key's
-// factors meet its score in fp32, with the sum of q for the offset.  A value's scale multiplies p, in fp32 before the rounding to
-// fp16; m is one reference a head for p and for that product, so that both stay in range.  The codes' middle is taken off the sums at
-// the end by the sum of the same rounded weights (one more MFMA a tile against a row of ones), and the offsets of the int4 kind add up to
-// one scalar a head.
+// factors meet its score in fp32, with the sum of q for the offset.  A value's scale multiplies p, in fp32 before the split in two; m is
+// one reference a head for p and for that product, so that both stay in range.  The codes' middle is taken off the sums at the end by
+// the sum of the same split weights (two more MFMAs a tile against a row of ones), and the offsets of the int4 kind add up to one scalar
+// a head.
 //
 // Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 74-77 us for 435 MB, 5.7-5.9 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
 // 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.5 us, all of it latency (the
@@ -50,8 +51,8 @@ static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start 
 // there are half as many shares (13 x up to 7411 int4: 21 us against 14).
 static constexpr long long PA_WIDE = 12288;
 
-// The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16 (int8 and int4 over 4 x 100001 tokens off
-// by 2.3e-4 of the output's norm, the output's own rounding 2.1e-4).
+// The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16, and the two numbers together are off by
+// at most 2^-33 of the largest weight where they are smaller still.
 static constexpr float PA_LIFT = 8.0f;
 static constexpr float PA_NEG = -1e30f;       // the reference before the first token: below every x, finite, so differences stay numbers
 
@@ -162,8 +163,9 @@ struct PaWave {
     struct Scores {
         float s[NS];
     };
-    // f16: the weights in two numbers of fp16, 22 bits, so that nothing but the output is rounded to 11 (off by 2.1e-4 of the output's
-    // norm, 2.7e-4 with one, in the same time: 2 x 131072 162 us); codes, whose arithmetic is dearer, in one (2.2e-4 to 2.5e-4).
+    // The weights in two numbers of fp16, 22 bits, so that nothing but the output is rounded to 11: off by 2.0e-4 to 2.1e-4 of the output's
+    // norm, as the output's rounding alone; with one number f16 2.7e-4, codes 2.2e-4 to 2.5e-4.  In the same time over f16 and int8 (2 x 131072
+    // f16 163 us; 32 x 1536 int8 20.3 us, 20.2 with one), dearer over int4 (4 x 100001 77.3 us, 76.6; 32 x 1536 14.7 us, 13.9).
     struct Weights {
         h8_t high, low;
     };
@@ -283,12 +285,16 @@ struct PaWave {
             l += p[j];
             if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(7.5f, vs[j], (float)fac.f[3][j]), zsum);
             pf[j] = (half_t)wt[j];
-            if constexpr (!CODES) rest[j] = (half_t)(wt[j] - (float)pf[j]);
+            rest[j] = (half_t)(wt[j] - (float)pf[j]);
         }
         if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
-            const u4_t w = __builtin_bit_cast(u4_t, pf);
             const uint32_t first = lane & 8 ? 0u : 0xFFFFFFFFu;
-            pf = __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
+            auto placed = [&](h8_t x) {
+                const u4_t w = __builtin_bit_cast(u4_t, x);
+                return __builtin_bit_cast(h8_t, u4_t{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first});
+            };
+            pf = placed(pf);
+            rest = placed(rest);
         }
         return {pf, rest};
     }
@@ -297,11 +303,13 @@ struct PaWave {
         for (int T = 0; T < OT; ++T) {
             const h8_t v = value_unit<KIND>(tile.v[T / n], T % n);
             acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.high, acc[T], 0, 0, 0);
-            if constexpr (!CODES) acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.low, acc[T], 0, 0, 0);
+            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.low, acc[T], 0, 0, 0);
         }
         if constexpr (CODES) {
             const half_t one = (half_t)1.0f;
-            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8_t{one, one, one, one, one, one, one, one}, w.high, psum, 0, 0, 0);
+            const h8_t ones = {one, one, one, one, one, one, one, one};
+            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w.high, psum, 0, 0, 0);
+            psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w.low, psum, 0, 0, 0);
         }
     }
     // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output: the offsets (of the
