@@ -70,8 +70,10 @@ __device__ __forceinline__ float over_groups(float v, F f) {
 __device__ __forceinline__ float group_max(float v) { return over_groups(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float group_sum(float v) { return over_groups(v, [](float a, float b) { return a + b; }); }
 
-// Eight halves of unit u (0 .. n - 1) of a 16-byte key chunk, element e times key_weight(e): the element itself, or its code u as
-// the subnormal u * 2^-24 (int4 elements 2, 3, 6, 7, masked where they stand: u * 2^-20, and q / 16 makes up for it).
+// Eight halves of unit u (0 .. n - 1) of a 16-byte key chunk: the elements, or their codes u as subnormals, u * 2^-24 (int8) or u * 2^-20
+// (int4, for the low bits that sums of subnormals lose: see value_unit).  All at one place, so that q enters as it is: a query is never
+// rounded (q / 16 for the nibbles that stand higher saves two shifts a unit, 32 x 1536 14.7 us for 14.9, but lost bits of queries
+// below 2^-10: outputs off by 3 % where all of q was about 1e-5).
 template <int KIND>
 __device__ __forceinline__ h8_t key_unit(const u4_t& c, int u) {
     u4_t o = c;
@@ -81,11 +83,11 @@ __device__ __forceinline__ h8_t key_unit(const u4_t& c, int u) {
         o[2] = __builtin_amdgcn_perm(0u, c[2 * u + 1], 0x0C010C00u);
         o[3] = __builtin_amdgcn_perm(0u, c[2 * u + 1], 0x0C030C02u);
     } else if constexpr (KIND == KMI_KV_INT4) {
-        const uint32_t w = c[u], w8 = w >> 8;
-        o[0] = w & 0x000F000Fu;
+        const uint32_t w = c[u];
+        o[0] = w << 4 & 0x00F000F0u;
         o[1] = w & 0x00F000F0u;
-        o[2] = w8 & 0x000F000Fu;
-        o[3] = w8 & 0x00F000F0u;
+        o[2] = w >> 4 & 0x00F000F0u;
+        o[3] = w >> 8 & 0x00F000F0u;
     }
     return __builtin_bit_cast(h8_t, o);
 }
@@ -113,13 +115,14 @@ struct PaWave {
     static constexpr int TILE_BYTES = kv_tile_bytes(D, KIND), PART = kv_part_bytes(D, KIND);
     static constexpr int NS = 8 / PACK;                        // scores a lane holds of a tile
     static constexpr bool CODES = KIND != KMI_KV_F16;
+    static constexpr float UNIT = !CODES ? 1.0f : KIND == KMI_KV_INT4 ? 0x1p20f : 0x1p24f;      // what a code's place divides it by
     typedef _Float16 fac_t __attribute__((ext_vector_type(NS)));
     h8_t q[PACK][KSTEPS];       // lane (column, g): q[32 kk + 8 g ..]
     f4_t acc[OT];               // lane (column, g): tile T = n c + a, rows dl = 4 g + r, d = 16 n c + n dl + a
     f4_t psum;                  // sum of the weights that entered acc (every row the same)
     float m;                    // the column's reference: weights are p = 2^(x - m), x = score * scale * log2(e)
     float l, zsum;              // this lane's share of the sums of p and of p * offset
-    float c, qc;                // scale * log2(e), for codes times 2^24 (their unit); sum of q, times scale * log2(e)
+    float c, qc;                // scale * log2(e) times UNIT; sum of q, times scale * log2(e)
 
     __device__ __forceinline__ void load_q(const half_t* qrow, bool used, int g) {
 #pragma unroll
@@ -129,14 +132,10 @@ struct PaWave {
         float s = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) {
-            h8_t x = q[0][kk];
+            const h8_t x = q[0][kk];
             if constexpr (CODES) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s += (float)x[e];
-            }
-            if constexpr (KIND == KMI_KV_INT4) {
-                const h8_t weight = {1.0f, 1.0f, 0.0625f, 0.0625f, 1.0f, 1.0f, 0.0625f, 0.0625f};
-                x = x * weight;
             }
             if constexpr (PACK == 1) {
                 q[0][kk] = x;
@@ -145,7 +144,7 @@ struct PaWave {
                 q[1][kk] = col < 8 ? h8_t{} : x;
             }
         }
-        c = CODES ? scale * 0x1p24f : scale;
+        c = scale * UNIT;
         qc = CODES ? group_sum(s) * scale : 0.0f;
 #pragma unroll
         for (int t = 0; t < OT; ++t) acc[t] = f4_t{};
@@ -320,7 +319,6 @@ struct PaWave {
         if constexpr (KIND == KMI_KV_INT8) add = -128.0f * psum[0];
         if constexpr (KIND == KMI_KV_INT4) add = group_sum(zsum) - 7.5f * psum[0];
     }
-    static constexpr float UNIT = !CODES ? 1.0f : KIND == KMI_KV_INT4 ? 0x1p20f : 0x1p24f;
     static __device__ __forceinline__ float other_half(float v) {          // row_ror 8: column c ^ 8 of the same lane group
         return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
     }

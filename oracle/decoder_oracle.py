@@ -178,3 +178,79 @@ def attend(q, k, v, scale):
     p = np.exp(s - s.max(-1, keepdims=True))
     t = p.sum(-1, keepdims=True)
     return p @ v / t, p @ np.abs(v) / t, t, p / t
+
+
+# ---- how far the kernel may be off ----------------------------------------------------------------------------------------
+MIDDLE = {"f16": 0.0, "int8": 128.0, "int4": 7.5}
+
+
+def sequence_codes(cache, page_row, first, length, head, D, kind):
+    """What the cache holds for positions first .. length - 1 of one head, taken apart: for keys and for values (codes [T, D], scale
+    [T], offset [T]), all fp64, so that the value is scale * (code - 128) (int8), scale * code + offset (int4), code (f16)."""
+    per = cache.shape[2]
+    t = np.arange(-(-length // TILE))
+    tiles = cache[np.asarray(page_row)[t // per], head, t % per]
+    get_tiles(tiles[:1], D, kind)
+    out = []
+    for part, at in enumerate(_PLACES[D, kind]):
+        byte, shift = at[..., 0], at[..., 1]
+        per_part = FACTORS[kind] // 2
+
+        def factor(i):
+            lo = np.array([factor_place(tau, i, D, kind) for tau in range(TILE)])
+            return np.stack((tiles[:, lo], tiles[:, lo + 1]), -1).view(np.float16)[..., 0].astype(np.float64).reshape(-1)[first:length]
+
+        if kind == "f16":
+            u = np.stack((tiles[:, byte], tiles[:, byte + 1]), -1).view(np.float16)[..., 0].astype(np.float64)
+            s, z = np.ones(length - first), np.zeros(length - first)
+        else:
+            u = ((tiles[:, byte].astype(np.int64) >> shift) & (255 if kind == "int8" else 15)).astype(np.float64)
+            s = factor(per_part * part)
+            z = factor(per_part * part + 1) if kind == "int4" else np.zeros(length - first)
+        out.append((u.reshape(-1, D)[first:length], s, z))
+    return out
+
+
+def attend_bound(q, keys, values, scale, kind, o, weights):
+    """How far decode attention may be off the exact outputs o [G, D] for the parts that sequence_codes gives; counts what the
+    kernel does, code by code:
+
+    A matrix instruction adds 32 products to an accumulator: taken as 33 terms brought to the largest one's exponent and cut to 24
+    bits, 33 * 2^-23 of the largest of them and of the sums before and behind.  A subnormal factor (codes enter as u * 2^-24, nibbles
+    as u * 2^-20) stands for 2^-14 in this: u as at least 1024, or 64.
+    Scores: D / 32 instructions, then the scale, and for codes the middle or the offset times the sum of q (D / 4 + 8 additions);
+    the exponent is rounded once or twice, exp2 and the references' changes cost 8 steps.  A score's error moves a weight by
+    as much, relative, and an output by that times the distance of the token's value.
+    Weights enter as two fp16 numbers: off by 2^-22 relative, or 2^-33 of the largest weight.
+    Sums: at least two waves take the tiles in turn, so T / 64 + 1 steps, each as above, over what is summed: the codes, and their
+    middle as often; the sums of p and of the offsets in fp32, 8 additions a step, and 16 for the joins.
+    Last the output's rounding."""
+    (ku, ks, kz), (vu, vs, vz) = keys, values
+    T, D = ku.shape
+    if T == 0:
+        return np.zeros(o.shape)
+    one, cut, mid = 2.0 ** -24, 33 * 2.0 ** -23, MIDDLE[kind]
+    least = {"f16": 2.0 ** -14, "int8": 1024.0, "int4": 64.0}[kind]
+    qd = q.astype(np.float64)
+    k = {"f16": ku, "int8": (ku - 128) * ks[:, None], "int4": ku * ks[:, None] + kz[:, None]}[kind]
+    v = {"f16": vu, "int8": (vu - 128) * vs[:, None], "int4": vu * vs[:, None] + vz[:, None]}[kind]
+    x = qd @ k.T * scale                                              # [G, T]
+    qn, kn = np.maximum(np.abs(qd), 2.0 ** -14), np.maximum(np.abs(ku), least)
+    run, err = np.zeros(x.shape), np.zeros(x.shape)
+    for at in range(0, D, 32):
+        before, run = run, run + qd[:, at:at + 32] @ ku[:, at:at + 32].T
+        term = (qn[:, None, at:at + 32] * kn[None, :, at:at + 32]).max(-1)
+        err += cut * np.maximum(term, np.maximum(np.abs(before), np.abs(run)))
+    offset = {"f16": 0.0 * ks, "int8": 128.0 * ks, "int4": np.abs(kz)}[kind]
+    err = scale * (ks * err + (D / 4 + 8) * one * np.abs(qd).sum(-1, keepdims=True) * offset
+                   + 8 * one * (ks * np.abs(run) + np.abs(qd.sum(-1, keepdims=True)) * offset))
+    err = err + one * (np.abs(x) + (x.max(-1, keepdims=True) - x) + 48) + 8 * 2 * one
+    assert (weights * err).max() < 0.1, "bound not meant for scores this coarse"
+    steps = T // 64 + 2
+    summed = weights @ (vs[:, None] * (np.abs(vu) + mid))
+    term = weights @ (vs[:, None] * np.maximum(np.abs(vu), least))
+    offsets = weights @ (mid * vs + np.abs(vz))
+    far = np.stack([(w * e) @ np.abs(v - c) for w, e, c in zip(weights, err, o)])
+    width = (vs[:, None] * np.abs(vu - mid)).max()
+    return (np.abs(o) * 2.0 ** -11 + 2.0 ** -25 + 1.1 * far + 2.0 ** -22 * (weights @ (vs[:, None] * np.abs(vu - mid))) + T * 2.0 ** -33 * width
+            + cut * (steps * summed + term) + (8 * steps + 16) * one * (np.abs(o) + offsets[:, None]))

@@ -36,3 +36,35 @@ def test_nothing_but_the_output_is_rounded_to_11_bits(ops, D, KV, G, kind):  # n
     step = np.spacing(np.abs(want).astype(np.float16)).astype(np.float64)
     off, rounding = np.sqrt(((got - want) ** 2).mean()), np.sqrt((step ** 2).mean() / 12)
     assert off <= 1.1 * rounding, (off, rounding)
+
+
+def check_close(cache, pages, lens, q, KV, D, kind, got, scale=None, window=0):
+    """Every output within what DO.attend_bound counts."""
+    G, sc = q.shape[1] // KV, D ** -0.5 if scale is None else scale
+    got = got.cpu().numpy().astype(np.float64)
+    for b, n in enumerate(lens):
+        lo = max(0, n - window) if window else 0
+        for h in range(KV):
+            if n == 0:
+                assert not got[b].any()
+                continue
+            k, v = DO.sequence(cache, pages[b], n, h, D, kind)
+            at = slice(h * G, (h + 1) * G)
+            o, _, _, w = DO.attend(q[b, at], k[lo:], v[lo:], sc)
+            bound = DO.attend_bound(q[b, at], *DO.sequence_codes(cache, pages[b], lo, n, h, D, kind), sc, kind, o, w)
+            off = np.abs(got[b, at] - o)
+            assert (off <= bound).all(), (b, h, n, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, G", [(64, 4), (128, 12), (256, 8)])
+@pytest.mark.parametrize("size, ksize", [(1e-3, 1.0), (3e-4, 12000.0), (2e-4, 1.0), (5e-5, 1.0), (1e-5, 1.0)])
+def test_small_queries_under_a_large_scale(ops, size, ksize, D, G, kind):  # noqa: F811
+    """Queries down to fp16's subnormal numbers, the scale (or the keys) as much larger: scores of a normal spread."""
+    lens = [300, 64]
+    rng = np.random.default_rng(D)
+    cache, pages = appended(ops, rng, lens, 1, D, kind, 32, size=ksize)
+    q = (rng.standard_normal((2, G, D)) * size).astype(np.float16)
+    scale = float(np.float32(2.0 / (size * ksize * D ** 0.5)))
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens), scale=scale)
+    check_close(cache.cpu().numpy(), pages, lens, q, 1, D, kind, got, scale)
