@@ -68,3 +68,51 @@ def test_small_queries_under_a_large_scale(ops, size, ksize, D, G, kind):  # noq
     scale = float(np.float32(2.0 / (size * ksize * D ** 0.5)))
     got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens), scale=scale)
     check_close(cache.cpu().numpy(), pages, lens, q, 1, D, kind, got, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, H, KV", [(64, 4, 4), (64, 20, 1), (128, 7, 1), (128, 8, 2), (128, 33, 1), (256, 16, 1), (256, 4, 2)])
+def test_ragged_lengths(ops, D, H, KV, kind):  # noqa: F811
+    """One token, none, a tile's edges, several tiles; query groups of 1, 4, 7, 16, 20 and 33."""
+    lens = [1, 0, 31, 32, 33, 100, 129]
+    rng = np.random.default_rng(D + H)
+    cache, pages = appended(ops, rng, lens, KV, D, kind, 64)
+    q = (rng.standard_normal((len(lens), H, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    check_close(cache.cpu().numpy(), pages, lens, q, KV, D, kind, got)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [1, 5, 77])
+def test_windows(ops, window, kind):  # noqa: F811
+    lens = [200, 64, 3, 0]
+    rng = np.random.default_rng(window)
+    cache, pages = appended(ops, rng, lens, 2, 64, kind, 96)
+    q = (rng.standard_normal((4, 8, 64)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens), scale=0.2, window=window)
+    check_close(cache.cpu().numpy(), pages, lens, q, 2, 64, kind, got, 0.2, window)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D, G, width", [(64, 4, None), (128, 8, None), (128, 20, 5000), (256, 4, None)])
+def test_sequences_cut_into_shares(ops, D, G, width, kind):  # noqa: F811
+    """Long ones cut and joined next to short ones; with a wide page table 32 query heads of a key head at once."""
+    lens = [2500, 1, 40, 1801]
+    rng = np.random.default_rng(D + G)
+    cache, pages = appended(ops, rng, lens, 1, D, kind, 32, width=width)
+    q = (rng.standard_normal((4, G, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    check_close(cache.cpu().numpy(), pages, lens, q, 1, D, kind, got)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_tasks(ops, kind):  # noqa: F811
+    """Two-wave workgroups: thousands of short tasks, one long one cut among them."""
+    D, G, B, KV = 64, 4, 260, 8
+    lens = [0 if i % 9 == 4 else 700 if i == 17 else 1 + (i * 23) % 45 for i in range(B)]
+    rng = np.random.default_rng(B)
+    cache, pages = appended(ops, rng, lens, KV, D, kind, 32)
+    q = (rng.standard_normal((B, G * KV, D)) * 2).astype(np.float16)
+    got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
+    some = [0, 4, 17, 100, B - 1]
+    check_close(cache.cpu().numpy(), pages[some], [lens[b] for b in some], q[some], KV, D, kind, got[some])
