@@ -355,7 +355,8 @@ int kmi_kv_read(const kmi_kv_read_args* args, void* stream);
 
 /* out fp16 [B][H][D] <- softmax(scale q . K) V over positions max(0, lens[b] - window) .. lens[b] - 1 (window 0: from 0) of the
  * cache, H a multiple of KV, query head h on key head h / (H / KV); q fp16 [B][H][D] with an element stride for B.  A sequence
- * of no tokens gives zeros; one longer than its row of the page table gives NaN.  0 < scale < 1e16.  The cache's length is split over
+ * of no tokens gives zeros; one longer than its row of the page table gives NaN.  Over an f16 cache an infinite value that counts gives
+ * that infinity, infinities of both signs NaN, scores that are all -infinity NaN, as the formula does.  0 < scale < 1e16.  The cache's length is split over
  * workgroups; the partial sums and arrival counters go to a workspace laid out and kept as kmi_gemv_w4a16's (a header of
  * KMI_GEMV_WS_HEADER bytes of counters, zero before the call and after it; KMI_PAGED_ATTN_WS bytes suffice for every shape): calls
  * that share one must be ordered, a call that did not run to completion is followed by kmi_gemv_ws_reset.  Results do not

@@ -69,6 +69,8 @@ __device__ __forceinline__ float over_groups(float v, F f) {
 }
 __device__ __forceinline__ float group_max(float v) { return over_groups(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float group_sum(float v) { return over_groups(v, [](float a, float b) { return a + b; }); }
+// What a sum is worth relative to a higher reference, 2^x.  Never zero: an infinite sum stays one, and 2^-126 of a finite one is nothing.
+__device__ __forceinline__ float decay(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
 
 // Eight halves of unit u (0 .. n - 1) of a 16-byte key chunk: the elements, or their codes u as subnormals, u * 2^-24 (int8) or u * 2^-20
 // (int4, for the low bits that sums of subnormals lose: see value_unit).  All at one place, so that q enters as it is: a query is never
@@ -104,6 +106,14 @@ __device__ __forceinline__ h8_t value_unit(const u4_t& c, int a) {
         if constexpr (KIND == KMI_KV_INT4) o[i] = (a == 0 ? c[i] << 4 : c[i] >> (4 * a - 4)) & 0x00F000F0u;
     }
     return __builtin_bit_cast(h8_t, o);
+}
+
+// Infinities and NaN to fp16's largest numbers, by the bits: as integers with a sign the positive ones stand highest, without one the negative.
+__device__ __forceinline__ h8_t in_range(h8_t x) {
+    typedef int16_t s8_t __attribute__((ext_vector_type(8)));
+    typedef uint16_t us8_t __attribute__((ext_vector_type(8)));
+    const s8_t p = __builtin_elementwise_min(__builtin_bit_cast(s8_t, x), (s8_t)(int16_t)0x7BFF);
+    return __builtin_bit_cast(h8_t, __builtin_elementwise_min(__builtin_bit_cast(us8_t, p), (us8_t)(uint16_t)0xFBFF));
 }
 
 // One wave's share of one head's tokens.  PACK = 2 (at most 8 query heads): columns 0-7 of the product are the heads on the tokens of
@@ -266,7 +276,7 @@ struct PaWave {
             }
             top = group_max(top);
             const float m2 = fmaxf(m, CODES ? fmaxf(group_max(wide) - PA_LIFT, top - 40.0f) : top - PA_LIFT);
-            const float a = __builtin_amdgcn_exp2f(m - m2);
+            const float a = decay(m - m2);
             m = m2;
             l *= a; zsum *= a;
             if constexpr (CODES) psum = psum * a;
@@ -284,6 +294,8 @@ struct PaWave {
             l += p[j];
             if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(7.5f, vs[j], (float)fac.f[3][j]), zsum);
             pf[j] = (half_t)wt[j];
+            // a token that counts has some weight, however low its score: an infinite value's weight never rounds to 0 (0 * inf)
+            if constexpr (!CODES) pf[j] = y[j] > -__builtin_inff() ? __builtin_fmaxf16(pf[j], (half_t)0x1p-24f) : pf[j];
             rest[j] = (half_t)(wt[j] - (float)pf[j]);
         }
         if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
@@ -297,12 +309,14 @@ struct PaWave {
         }
         return {pf, rest};
     }
+    // f16: the low numbers are of either sign or zero, so they meet the values brought into fp16's range, and an infinite value comes through
+    // the high numbers alone (as it is; of both signs NaN).  Two packed instructions for two values: 2 x 131072 162.9 us, 162.3 without.
     __device__ __forceinline__ void add(const Tile& tile, const Weights& w) {
 #pragma unroll
         for (int T = 0; T < OT; ++T) {
             const h8_t v = value_unit<KIND>(tile.v[T / n], T % n);
             acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.high, acc[T], 0, 0, 0);
-            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.low, acc[T], 0, 0, 0);
+            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(CODES ? v : in_range(v), w.low, acc[T], 0, 0, 0);
         }
         if constexpr (CODES) {
             const half_t one = (half_t)1.0f;
@@ -425,12 +439,12 @@ __device__ __forceinline__ void join_shares(const float* partial, int slot, int 
                     m[k] = v + k * dealt < here ? held[2 * ((v + k * dealt) * COLS + c)] : PA_NEG;
                     next = fmaxf(next, m[k]);
                 }
-                const float keep = __builtin_amdgcn_exp2f(top - next);
+                const float keep = decay(top - next);
                 sum *= keep; o = o * keep; top = next;
 #pragma unroll
                 for (int k = 0; k < FLIGHT; ++k) {
                     if (v + k * dealt >= here) continue;
-                    const float f = __builtin_amdgcn_exp2f(m[k] - next);
+                    const float f = decay(m[k] - next);
                     sum += f * held[2 * ((v + k * dealt) * COLS + c) + 1];
                     o = o + y[k] * f;
                 }
@@ -448,7 +462,7 @@ __device__ __forceinline__ void join_shares(const float* partial, int slot, int 
             if (mine && first == 0) {
                 for (int k = 1; k < dealt; ++k) {
                     const float m = tops[2 * (k * quads + q)], next = fmaxf(top, m);
-                    const float keep = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+                    const float keep = decay(top - next), f = decay(m - next);
                     sum = sum * keep + f * tops[2 * (k * quads + q) + 1];
                     o = o * keep + outs[k * quads + q] * f;
                     top = next;
@@ -456,7 +470,7 @@ __device__ __forceinline__ void join_shares(const float* partial, int slot, int 
             }
         }
         if (mine && first == 0) {
-            const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float norm = 1.0f / sum;
             typedef _Float16 h4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<h4*>(out + 4 * q) = h4{(half_t)(o[0] * norm), (half_t)(o[1] * norm), (half_t)(o[2] * norm), (half_t)(o[3] * norm)};
         }
@@ -634,12 +648,12 @@ __global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void 
             if constexpr (PACK == 2) mm = fmaxf(mm, W::other_half(mm));
 #pragma unroll
             for (int v = 0; v < NW; ++v) {
-                a[v] = __builtin_amdgcn_exp2f(join.m[v][col] - mm);
+                a[v] = decay(join.m[v][col] - mm);
                 ll += a[v] * join.l[v][col];
                 plus += a[v] * join.add[v][col];
             }
             if constexpr (PACK == 2) { ll += W::other_half(ll); plus += W::other_half(plus); }
-            const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const float norm = 1.0f / ll;                      // 0 / 0 = NaN where every score is -inf
             float* part = slot + x * (32 + 16 * D);
             if (wave * MINE < W::OT) {
 #pragma unroll

@@ -374,7 +374,8 @@ def paged_attention(q, cache, page_table, lens, scale=None, window=0):
 
     H is a multiple of the cache's kv_heads (query head h reads key head h // (H / kv_heads)); lens int32 [B]; scale D^-0.5 by
     default; window > 0: the last `window` positions only.  A sequence of no tokens gives zeros; one longer than its row of
-    the page table, or with a page that is not one of the cache, NaN."""
+    the page table, or with a page that is not one of the cache, NaN.  An infinite value in an f16 cache comes through as the formula
+    has it (both signs, or no score above -infinity: NaN)."""
     D, kind = _cache_form(cache, "paged_attention")
     dev = cache.device
     if q.dim() == 3:

@@ -116,3 +116,65 @@ def test_many_tasks(ops, kind):  # noqa: F811
     got = ops.paged_attention(dev(q), cache, dev(pages), i32(*lens))
     some = [0, 4, 17, 100, B - 1]
     check_close(cache.cpu().numpy(), pages[some], [lens[b] for b in some], q[some], KV, D, kind, got[some])
+
+
+@pytest.mark.parametrize("D, G, width, size", [(64, 1, None, 2.0), (64, 4, None, 30.0), (128, 20, 5000, 2.0), (128, 4, None, 6.0), (256, 4, None, 2.0)])
+def test_infinite_values_come_through(ops, D, G, width, size):  # noqa: F811
+    """f16: an infinity that counts gives that infinity however small its weight -- in another wave's or share's tiles than a score e^300 times
+    as large, a lone token's whose weight is a power of two -- both signs or a NaN give NaN; the elements beside it stay as exact as ever."""
+    lens = [1, 40, 300, 2500]
+    rng = np.random.default_rng(D + G)
+    cache, pages = appended(ops, rng, lens, 1, D, "f16", 32, width=width)
+    host, q = cache.cpu().numpy(), (rng.standard_normal((4, G, D)) * size).astype(np.float16)
+    plain = {}
+    for b, n in enumerate(lens):
+        k, v = (x.astype(np.float16) for x in DO.sequence(host, pages[b], n, 0, D, "f16"))
+        plain[b] = v.copy()
+        if n > 1:                                                     # one token e^300 above the others for the first head
+            first = q[b, 0].astype(np.float64)
+            k[7] = (first * 300 * D ** 0.5 / (first @ first)).astype(np.float16)
+        low = int((q[b, -1].astype(np.float64) @ k.T.astype(np.float64)).argmin())
+        v[rng.integers(n), 0] = np.inf
+        v[low, 1] = -np.inf
+        v[n // 2, 2] = -np.inf; v[n - 1, 3] = np.inf
+        v[:, 4] = np.inf
+        v[n // 3, 5] = np.nan
+        v[0, 6] = np.inf; v[n - 1, 6] = -np.inf if n > 1 else np.inf
+        for t in range(n):
+            DO.put_token(host[pages[b, t // 32], 0, 0], t % 32, k[t], v[t], "f16")
+    got = ops.paged_attention(dev(q), dev(host), dev(pages), i32(*lens)).cpu().numpy().astype(np.float64)
+    for b, n in enumerate(lens):
+        k, v = DO.sequence(host, pages[b], n, 0, D, "f16")
+        with np.errstate(invalid="ignore"):
+            o, _, _, w = DO.attend(q[b], k, v, D ** -0.5)
+        assert (w > 0).all()
+        assert np.isposinf(o[:, [0, 3, 4]]).all() and np.isneginf(o[:, 1:3]).all() and np.isnan(o[:, 5]).all()
+        assert np.array_equal(got[b, :, :7], o[:, :7], equal_nan=True), (b, got[b, :, :7])
+        parts = [(k, np.ones(n), np.zeros(n)), (np.where(np.isfinite(v), v, 0.0), np.ones(n), np.zeros(n))]
+        o = w @ parts[1][0]
+        bound = DO.attend_bound(q[b], *parts, D ** -0.5, "f16", o, w)
+        assert (np.abs(got[b] - o)[:, 7:] <= bound[:, 7:]).all(), b
+
+
+def test_scores_of_minus_infinity(ops):  # noqa: F811
+    """f16: a token whose score is -inf has no weight at all; where every token's is, the output is NaN, not zero."""
+    D, G, lens = 64, 4, [1, 33, 33, 1700]
+    rng = np.random.default_rng(8)
+    cache, pages = appended(ops, rng, lens, 1, D, "f16", 32)
+    host, q = cache.cpu().numpy(), (rng.standard_normal((4, G, D)) * 2).astype(np.float16)
+    q[:, :, 0] = np.abs(q[:, :, 0]) + np.float16(1)
+    for b, n in enumerate(lens):
+        k, v = (x.astype(np.float16) for x in DO.sequence(host, pages[b], n, 0, D, "f16"))
+        out = slice(0, n) if b != 2 else slice(0, n - 1, 3)
+        k[out, 0] = -np.inf
+        for t in range(n):
+            DO.put_token(host[pages[b, t // 32], 0, 0], t % 32, k[t], v[t], "f16")
+    got = ops.paged_attention(dev(q), dev(host), dev(pages), i32(*lens))
+    assert torch.isnan(got[[0, 1, 3]]).all()
+    n = lens[2]
+    k, v = DO.sequence(host, pages[2], n, 0, D, "f16")
+    keep = np.isfinite(k[:, 0])
+    assert not keep[0] and keep[1]
+    parts = [(x[keep], np.ones(keep.sum()), np.zeros(keep.sum())) for x in (k, v)]
+    o, _, _, w = DO.attend(q[2], k[keep], v[keep], D ** -0.5)
+    assert (np.abs(got[2].cpu().numpy() - o) <= DO.attend_bound(q[2], *parts, D ** -0.5, "f16", o, w)).all()
