@@ -528,7 +528,8 @@ __global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void 
     // the row that the shares are cut from: pieces, one a share, or tiles and PA_TASK_COST a task, `quota` a share
     auto room = [&](int n) { return n == 0 ? 0 : even ? pieces_of(n, quota) : n + PA_TASK_COST; };     // a task's, in the row
     constexpr int SMALL = PA_WHOLE_STEPS * NW < PA_SMALL_BYTES / W::TILE_BYTES ? PA_WHOLE_STEPS * NW : PA_SMALL_BYTES / W::TILE_BYTES;
-    const int per_share = even ? 1 : quota, begin = run * per_share, end = begin + per_share;
+    // (workgroups past the last share own nothing: a multiple of their number would pass 2^31 where the row holds over 2^30 tiles)
+    const int per_share = even ? 1 : quota, begin = min(run, shares) * per_share, end = run < shares ? begin + per_share : begin;
     int b = p.B, before = 0;                                               // before: the room of the sequences in front
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int mine = room(tiles_of(b0)) * sp.tasks_a_sequence, upto = wave_scan(mine);

@@ -178,3 +178,23 @@ def test_scores_of_minus_infinity(ops):  # noqa: F811
     parts = [(x[keep], np.ones(keep.sum()), np.zeros(keep.sum())) for x in (k, v)]
     o, _, _, w = DO.attend(q[2], k[keep], v[keep], D ** -0.5)
     assert (np.abs(got[2].cpu().numpy() - o) <= DO.attend_bound(q[2], *parts, D ** -0.5, "f16", o, w)).all()
+
+
+def test_a_row_of_over_a_billion_tiles(ops):  # noqa: F811
+    """1000 sequences of 34 million tokens that share their pages, 256 shares of the work for 512 workgroups: twice the quota times
+    256 passes 2^31, so the workgroups past the last share must not multiply by it.  Equal scores, value scales and codes that are
+    powers of two: every sum is exact (at most 2^24 equal terms a lane), and so is the output."""
+    B, D, G, tiles, width = 1000, 64, 8, 1024, 1055
+    length = 32 * (tiles * width - 256)
+    units = B * (length // 32)
+    assert 2 ** 30 < units and 511 * (units // 256) >= 2 ** 31 and B * (tiles * width + 6) <= 0x7FFF0000
+    cache = torch.full((2, 1, tiles, ops.kv_tile_bytes(D, "int8")), 64, dtype=torch.uint8, device="cuda")
+    for page in range(2):
+        factors = torch.tensor([1.0, 2.0 ** (page - 6)], dtype=torch.float16, device="cuda").repeat_interleave(32)
+        cache[page, 0, :, 4 * 32 * D // 2:] = factors.view(torch.uint8)
+    pages = (torch.arange(B, dtype=torch.int32, device="cuda") % 2)[:, None].repeat(1, width)
+    q, lens = torch.zeros((B, G, D), dtype=torch.float16, device="cuda"), torch.full((B,), length, dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, cache, pages, lens)
+    want = -(2.0 ** (torch.arange(B, device="cuda") % 2))                  # (64 - 128) * 2^(page - 6)
+    assert (got.float() == want[:, None, None]).all()
+    assert not ops.gemv_workspace_for("cuda")[:65536].any()
