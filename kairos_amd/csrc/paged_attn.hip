@@ -225,6 +225,7 @@ struct PaWave {
     // is 2^8, or the largest p 2^40 where every value scale is tiny) only where a weight would pass 2^15 or p 2^48, which is seldom
     // after a wave's first tile: no reduction over lanes otherwise.  fac: the tile's factors, tok: its first token, [lo, hi) the
     // tokens that count, bad: no page of this cache.
+    template <bool CAREFUL>
     __device__ __forceinline__ Weights weights(const Scores& sc, Tile& tile, Factors& fac, int tok, int lo, int hi, bool bad, int lane) {
         float vs[NS], y[NS], p[NS], wt[NS];
 #pragma unroll
@@ -294,8 +295,8 @@ struct PaWave {
             l += p[j];
             if constexpr (KIND == KMI_KV_INT4) zsum = __builtin_fmaf(p[j], __builtin_fmaf(7.5f, vs[j], (float)fac.f[3][j]), zsum);
             pf[j] = (half_t)wt[j];
-            // a token that counts has some weight, however low its score: an infinite value's weight never rounds to 0 (0 * inf)
-            if constexpr (!CODES) pf[j] = y[j] > -__builtin_inff() ? __builtin_fmaxf16(pf[j], (half_t)0x1p-24f) : pf[j];
+            // careful: a token that counts has some weight, however low its score, so that an infinite value's never rounds to 0 (0 * inf)
+            if constexpr (CAREFUL) pf[j] = y[j] > -__builtin_inff() ? __builtin_fmaxf16(pf[j], (half_t)0x1p-24f) : pf[j];
             rest[j] = (half_t)(wt[j] - (float)pf[j]);
         }
         if constexpr (PACK == 2) {                             // the lane's tokens are its column's half of the operand's eight
@@ -309,14 +310,15 @@ struct PaWave {
         }
         return {pf, rest};
     }
-    // f16: the low numbers are of either sign or zero, so they meet the values brought into fp16's range, and an infinite value comes through
-    // the high numbers alone (as it is; of both signs NaN).  Two packed instructions for two values: 2 x 131072 162.9 us, 162.3 without.
+    // Careful: the low numbers are of either sign or zero, so they meet the values brought into fp16's range, and an infinite value comes
+    // through the high numbers alone (as it is; of both signs NaN).
+    template <bool CAREFUL>
     __device__ __forceinline__ void add(const Tile& tile, const Weights& w) {
 #pragma unroll
         for (int T = 0; T < OT; ++T) {
             const h8_t v = value_unit<KIND>(tile.v[T / n], T % n);
             acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w.high, acc[T], 0, 0, 0);
-            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(CODES ? v : in_range(v), w.low, acc[T], 0, 0, 0);
+            acc[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(CAREFUL ? in_range(v) : v, w.low, acc[T], 0, 0, 0);
         }
         if constexpr (CODES) {
             const half_t one = (half_t)1.0f;
@@ -324,6 +326,13 @@ struct PaWave {
             psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w.high, psum, 0, 0, 0);
             psum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w.low, psum, 0, 0, 0);
         }
+    }
+    // Is there a sum that is not finite while the weights are numbers?
+    __device__ __forceinline__ bool not_finite() const {
+        f4_t s = f4_t{};
+#pragma unroll
+        for (int T = 0; T < OT; ++T) s = s + acc[T] * 0.0f;
+        return __any(!(s[0] + s[1] + s[2] + s[3] == 0.0f) && l == l);
     }
     // What the join needs besides m and acc: the sums over the lane groups, and what is added to every output: the offsets (of the
     // codes' middle), less the middle times the very weights that entered acc, so that their rounding cancels.
@@ -608,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void 
 #pragma unroll
         for (int x = 0; x < HT; ++x) w[x].start(col, sp.c);
         // (a load under a condition would make the compiler wait for every load wherever it waits for one)
-        auto step = [&](auto more, int i) {
+        auto step = [&](auto more, auto careful, int i) {
             typename W::Scores sc[HT];
 #pragma unroll
             for (int x = 0; x < HT; ++x) sc[x] = w[x].scores(tile, lane);
@@ -619,16 +628,32 @@ __global__ __launch_bounds__(64 * NW, NW * pa_a_cu(D, KIND, PACK, NW) / 4) void 
             typename W::Weights o[HT];
 #pragma unroll
             for (int x = 0; x < HT; ++x)
-                o[x] = w[x].weights(sc[x], tile, fac, (seq.first + ta + wave + NW * i) * KV_TILE, seq.lo, seq.hi, bad, lane);
+                o[x] = w[x].template weights<careful.value>(sc[x], tile, fac, (seq.first + ta + wave + NW * i) * KV_TILE, seq.lo, seq.hi, bad, lane);
             __builtin_amdgcn_sched_barrier(0);                 // values are decoded where they are used: not before, into registers
 #pragma unroll
-            for (int x = 0; x < HT; ++x) w[x].add(tile, o[x]);
+            for (int x = 0; x < HT; ++x) w[x].template add<careful.value>(tile, o[x]);
             if constexpr (more.value) fetch_values();
             __builtin_amdgcn_sched_barrier(0);
         };
         int i = 0;
-        for (; i + 1 < count; ++i) step(Flag<true>(), i);
-        if (i < count) step(Flag<false>(), i);
+        for (; i + 1 < count; ++i) step(Flag<true>(), Flag<false>(), i);
+        if (i < count) step(Flag<false>(), Flag<false>(), i);
+        if constexpr (!W::CODES) {
+            // f16: infinities or NaN among the values.  The wave's tiles once more, carefully: two packed instructions for two values, which
+            // one wave a SIMD does not hide (1 x 1152 11.4 us for 10.2 if all tiles were taken so), and no loads ahead.
+            bool again = false;
+#pragma unroll
+            for (int x = 0; x < HT; ++x) again |= w[x].not_finite();
+            if (again) {
+#pragma unroll
+                for (int x = 0; x < HT; ++x) w[x].start(col, sp.c);
+                for (i = 0; i < count; ++i) {
+                    fetch_keys(i);
+                    fetch_values();
+                    step(Flag<false>(), Flag<true>(), i);
+                }
+            }
+        }
 
         // the waves' sums, joined
         const bool complete = parts == 1;
