@@ -13,18 +13,18 @@
 // the sum of the same split weights (two more MFMAs a tile against a row of ones), and the offsets of the int4 kind add up to one scalar
 // a head.
 //
-// Bound by the reading of the cache: 4 x 100001 int4 (64 heads on 8 of 128) 74-77 us for 435 MB, 5.7-5.9 TB/s; 2 x 131072 f16 (1074 MB) 161 us,
-// 6.7 TB/s; 64 ragged up to 8192 f16 93 us, 6.0 TB/s; 32 x 1536 int8 20.0 us.  One sequence of 200 tokens: 6.5 us, all of it latency (the
-// schedule 2, the first loads 1, the joins 2).
+// Bound by the reading of the cache (a plain read past the caches: 7.0 TB/s): 2 x 131072 f16 (1074 MB) 162 us, 6.6 TB/s; 64 ragged up to 8192
+// f16 95 us, 5.8 TB/s; 32 x 1536 int8 20.4 us; over int4 by its arithmetic as well: 4 x 100001 (64 heads on 8 of 128) 76-77 us for 435 MB,
+// 5.7 TB/s.  One sequence of 200 tokens: 6.7-6.9 us, all of it latency (the schedule 2, the first loads 1, the joins 2).
 #include "kv_parts.h"
 
 // Waves of a workgroup.  Loads are short of flight where tiles are small, so there eight waves (two a SIMD, one computing while the other
-// waits): int4 (4 x 100001: 76 us, four waves 95), int8 with heads of 64 (8 x 60000: 84 us, 100), and 32 query heads a wave, for their
-// arithmetic (64 x 62479 int8, 20 heads: 91 us, 110).  Else four read as fast and start and end a share sooner (1 x 4096 int8:
-// 11.2 us, 13.6).  More tasks than CUs: small workgroups, several a CU, so that one task's end hides behind another's middle:
-// int4 of 128 with over 256 tasks four waves (64 x up to 1000, 8 key heads: 14 us, 30 with eight; up to 8000: 64, 79; but 256
-// tasks, 32 x 1536: 20, 14 with eight); from 2048 on, or 1024 of codes with heads of 64, two (256 x up to 300, 8 key heads of 128,
-// int8: 30 us, 40 with four; 1000 x up to 100 int4: 60, 83; against it 256 x up to 2000 f16: 184, 172).  Heads of 256 fill a SIMD's
+// waits): int4 (4 x 100001: 77 us, four waves 85), int8 with heads of 64 (8 x 60000: 82 us, 97), and 32 query heads a wave, for their
+// arithmetic (64 x up to 62479 int8, 20 heads of 64: 66 us, 78).  Else four read as fast and start and end a share sooner (1 x 4096 int8:
+// 11.5 us, 14.2).  More tasks than CUs: small workgroups, several a CU, so that one task's end hides behind another's middle:
+// int4 of 128 with over 256 tasks four waves (64 x up to 1000, 8 key heads: 15.4 us, 28 with eight; up to 8000: 63, 83; but 256
+// tasks, 32 x 1536: 23.5, 15.6 with eight); from 2048 on, or 1024 of codes with heads of 64, two (256 x up to 300, 8 key heads of 128,
+// int8: 29 us, 40 with four; 1000 x up to 100 int4: 63, 86; against it 256 x up to 2000 f16: 184, 172).  Heads of 256 fill a SIMD's
 // registers with one wave.
 static constexpr bool pa_codes64(int D, int kind, int pack) { return kind != KMI_KV_F16 && D == 64 && pack == 2; }
 static int pa_waves(int D, int kind, int pack, int columns, long long tasks) {
@@ -37,8 +37,8 @@ static constexpr int pa_a_cu(int D, int kind, int pack, int waves) {         // 
     const int most = D == 256 ? 4 : pa_codes64(D, kind, pack) ? 16 : kind == KMI_KV_INT4 && pack == 2 ? 12 : 8;      // waves
     return most < waves ? 1 : most / waves;
 }
-// Shares.  256 at a time, one a CU, read a long cache 5 % faster than 512 (161 us against 169 for 2 x 131072 f16: fewer places of
-// memory at once), more hide the starts and ends of short tasks (64 x up to 1000 int8, 8 key heads: 18.5 us, 29 with 256 workgroups).
+// Shares.  256 at a time, one a CU, read a long cache 4 % faster than 512 (164 us against 170 for 2 x 131072 f16: fewer places of
+// memory at once), more hide the starts and ends of short tasks (64 x up to 1000 int8, 8 key heads: 19 us, 28 with 256 workgroups).
 static constexpr int PA_LONG = 96;            // tiles a share from which 256 uneven ones are taken all the same
 // Being cut costs a task about 3 us (hand-off and join): none of up to nine tiles a wave is (2 x 1152 f16, 36 tiles: 9.6 us
 // whole, 10.6 cut), and no share is smaller than three (1 x 4096 f16: 11.8 us, 13.2 with six).
@@ -47,8 +47,9 @@ static constexpr int PA_SMALL_BYTES = 320 << 10;   // of a task that no row of t
 static constexpr int PA_HELD = 1024;          // sequences whose lengths the schedule keeps in LDS
 static constexpr int PA_TASK_COST = 6;        // tiles' worth of a task's start and end; 3 and 12 measured the same
 // Tiles of the page table from which a wave takes 32 query heads at once (more than 16 share a key head; not int4, whose arithmetic
-// then spills: 40 us against 30): the cache is read once (16 x up to 20000 f16, 64 heads on 2: 43 us against 63; int8 33 and 40), but
-// there are half as many shares (13 x up to 7411 int4: 21 us against 14).
+// then spills: 40 us against 30): the cache is read once (16 x up to 20000 f16, 64 heads on 2: 44 us against 63; int8 34 and 41), but
+// there are half as many shares (13 x up to 7411 int4: 21 us against 14).  By the table's room, since the lengths are on the device: short
+// sequences under a wide table take this form too.
 static constexpr long long PA_WIDE = 12288;
 
 // The largest weight starts at 2^8: weights down to 2^-22 of it are then normal numbers of fp16, and the two numbers together are off by
@@ -181,7 +182,7 @@ struct PaWave {
     // The first of the lane's NS tokens in a tile.
     static __device__ __forceinline__ int first_token(int lane) { return 8 * (lane >> 4) + (PACK == 2 ? (lane >> 1) & 4 : 0); }
 
-    // A cache is read once a step: loads that leave nothing behind in the caches (2 x 131072 f16: 161 us, 182 with ordinary ones; 64 ragged up
+    // A cache is read once a step: loads that leave nothing behind in the caches (2 x 131072 f16: 162 us, 182 with ordinary ones; 64 ragged up
     // to 8192: 93, 107; against it a cache small enough to stay: 8 x up to 3000 f16, heads of 256: 27, 20).
     static __device__ __forceinline__ void load_keys(Tile& t, const char* tile, int lane) {
 #pragma unroll

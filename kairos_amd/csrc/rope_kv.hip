@@ -10,8 +10,9 @@
 // tiny row (subnormal s) is clipped.  The quotients and the reciprocal are IEEE divisions, every step is rounded to fp32
 // once: the codes are the same on any machine.  A row with an infinity or NaN gets the scale NaN and reads as NaN.
 // Traffic: every row read once and written once, plus the table's R * 4 bytes a token; bound by the memory.  Measured: rotation
-// alone, 4 x 4001 tokens, 28 + 4 heads of 128: 50 us for 262 MB, 5.2 TB/s (a large copy: 5.0); into the cache, 32 x 1024 tokens, 32 + 8 + 8
-// heads of 128: int4 158 us for 707 MB, 4.5 TB/s; 3 x 777 tokens, 64 + 8 + 8 heads, f16: 22 us for 96 MB, 4.4 TB/s; one token of 32 sequences: 4 us.
+// alone, 4 x 4001 tokens, 28 + 4 heads of 128: 51 us for 263 MB, 5.2 TB/s (a large copy: 5.0); into the cache, 32 x 1024 tokens, 32 + 8 + 8
+// heads of 128: int4 164 us (155 at best) for 707 MB, 4.3 TB/s; 3 x 777 tokens, 64 + 8 + 8 heads, f16: 23 us for 96 MB, 4.2 TB/s; one token of
+// 32 sequences: 4 us.
 #include "kv_parts.h"
 #include <type_traits>
 
@@ -409,7 +410,7 @@ __device__ __forceinline__ h8_t unpack_row(const Packed<KIND>& w, float s, float
 
 // One workgroup: eight neighbouring positions 8 i .. 8 i + 7 of one sequence, 2048 / D rows (key heads, then value heads); a lane
 // reads eight elements of one row of all eight tokens (whole chunks of values, turned over in registers).  Bound by the memory: 16 x
-// 8000 tokens, 8 heads of 64, int4: 62 us for 336 MB, 5.4 TB/s (107 us a token at a time; 76 with stores that stay in the caches, against
+// 8000 tokens, 8 heads of 64, int4: 61 us for 336 MB, 5.5 TB/s (107 us a token at a time; 76 with stores that stay in the caches, against
 // loads past them 117: two lanes' loads share a line).
 template <int D, int KIND>
 __global__ __launch_bounds__(256) void kv_read_kernel(kmi_kv_read_args p) {
